@@ -247,19 +247,15 @@ def _plain_reorder(s):
 def _plain_reserve(s):
     count, columns = s.tables.shape
     pages, page = s.refs.shape[0], s.page
-    row, column = _index(count), _index(columns)
+    column = _index(columns)
     length, new, tables = s.lengths.long(), s.counts.long(), s.tables.long()
     bad = (new < 0) | (length < 0) | (length + new > columns * page)
     new = torch.where(bad, 0, new)
     first, end = length // page, length + new
     current = tables.gather(1, first.clamp(0, columns - 1)[:, None])[:, 0]
-    holders = s.refs.long()[current.clamp(min=0)]
-    shared = (new > 0) & (current >= 0) & (holders > 1)
-    same = (current[:, None] == current[None]) & shared[:, None] & shared[None]
-    earlier = (same & (row[None] < row[:, None])).any(1)
-    moves = shared & ~((same.sum(1) == holders) & ~earlier)
+    shared = (new > 0) & (current >= 0) & (s.refs[current.clamp(min=0)] > 1)
     written = (column[None] >= first[:, None]) & (column[None] * page < end[:, None]) & (new > 0)[:, None]
-    need = written & ((tables < 0) | (moves[:, None] & (column[None] == first[:, None])))
+    need = written & ((tables < 0) | (shared[:, None] & (column[None] == first[:, None])))
     wants = need.sum(1)
     free = (s.refs == 0).sum()
     short = (wants > 0) & (wants.cumsum(0) > free)
@@ -268,7 +264,7 @@ def _plain_reserve(s):
     order = torch.argsort((s.refs != 0).int(), stable=True)  # the free pages, lowest first
     rank = need.flatten().long().cumsum(0) - 1
     given = torch.where(need & take[:, None], order[rank.clamp(0, pages - 1)].view(count, columns), -1)
-    leave = moves & take
+    leave = shared & take
     s.refs.index_add_(0, current.clamp(min=0), -leave.int())
     s.refs.index_add_(0, given.clamp(min=0).flatten(), (given >= 0).int().flatten())
     tables = torch.where(given >= 0, given, tables)
