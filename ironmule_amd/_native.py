@@ -26,7 +26,8 @@ LIB_PATH = os.path.join(PKG, "libironmule_qmv.so")
 HEADER_PATH = os.path.join(ROOT, "include", "ironmule_qmv.h")
 HEADER_PATHS = [HEADER_PATH, os.path.join(ROOT, "include", "ironmule_decode.h"),
                 os.path.join(ROOT, "include", "ironmule_step.h"),
-                os.path.join(ROOT, "include", "ironmule_prompt.h")]
+                os.path.join(ROOT, "include", "ironmule_prompt.h"),
+                os.path.join(ROOT, "include", "ironmule_paged.h")]
 
 GROUP_SIZE = 64
 BITS = 4
@@ -110,6 +111,20 @@ class PromptShape(ctypes.Structure):
                 ("theta", ctypes.c_double)]
 
 
+class PagedCacheDesc(ctypes.Structure):
+    """imq_paged_cache: the tables, lengths and page references of a paged cache."""
+
+    _fields_ = [("tables", _P), ("lengths", _P), ("refs", _P), ("requests", _I32), ("columns", _I32), ("pages", _I32),
+                ("page_size", _I32)]
+
+
+class PagedChunkDesc(ctypes.Structure):
+    """imq_paged_chunk: what a reservation gives the rows of a step."""
+
+    _fields_ = [("starts", _P), ("ends", _P), ("status", _P), ("positions", _P), ("slots", _P), ("copies", _P),
+                ("rows", _I32)]
+
+
 class QmvStage(ctypes.Structure):
     """imq_qmv_stage: 1-3 one-row qmv problems sharing x, optionally after the previous stage."""
 
@@ -182,6 +197,17 @@ _SIGNATURES = {
     "imq_prompt_layer": ([ctypes.POINTER(StepLayer), ctypes.POINTER(PromptShape), _P, _I32, _P, ctypes.c_size_t, _P],
                          _I32),
     "imq_prompt_finish": ([ctypes.POINTER(PromptShape), _P, _I32, _P, ctypes.c_size_t, _P], _I32),
+    # paged caches and beams (include/ironmule_paged.h)
+    "imq_paged_reserve": ([ctypes.POINTER(PagedCacheDesc), _P, ctypes.POINTER(PagedChunkDesc), _P, _I32, _I64, _P], _I32),
+    "imq_paged_reorder": ([ctypes.POINTER(PagedCacheDesc), _P, _P], _I32),
+    "imq_paged_write": ([_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _I64, _P, _P, _I32, _I32, _I32, _I32, _I32,
+                         _I32, ctypes.c_double, ctypes.c_float, _P], _I32),
+    "imq_paged_attention_workspace": ([_I32] * 7, ctypes.c_size_t),
+    "imq_paged_attention": ([_P, _I64, _P, _P, _P, _P, _P, _P, _I64] + [_I32] * 10 + [ctypes.c_float, _P, ctypes.c_size_t,
+                                                                                     _P], _I32),
+    "imq_beam_select_workspace": ([_I32] * 4, ctypes.c_size_t),
+    "imq_beam_select": ([_P, _I64, _I32, _P, _P, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, ctypes.c_size_t, _P],
+                        _I32),
     # persistent programs (include/ironmule_step.h)
     "imq_decode_program_create": ([ctypes.POINTER(StepDesc), ctypes.POINTER(_P)], _I32),
     "imq_qmv_program_create": ([ctypes.POINTER(QmvStage), _I32, ctypes.POINTER(_P)], _I32),
@@ -661,6 +687,192 @@ class PromptLayers:
         _check(lib().imq_prompt_finish(ctypes.byref(self.shape), _ptr(self.h), 1, _ptr(self.workspace), self.nbytes,
                                        _stream(None)))
         return self.h[-1:]
+
+
+# --------------------------------------------------------------- paged caches and beams
+
+MAX_PAGED_REQUESTS = 1024
+MAX_BEAMS = 64
+MAX_CONTINUATIONS = 64
+
+
+def _current_gpu(*tensors: torch.Tensor) -> int:
+    """The current GPU's index, where every tensor has to be: these calls run on its current stream."""
+    index = tensors[0].get_device()
+    if index < 0:
+        raise ValueError("the tensors must be on a GPU")
+    if index != torch._C._cuda_getDevice():
+        raise ValueError(f"the tensors are on GPU {index}, which is not the current one")
+    _same_device(index, *tensors)
+    return index
+
+
+def _ints(name: str, t: torch.Tensor, *shape: int) -> None:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _cache_desc(tables, lengths, refs, page_size: int) -> PagedCacheDesc:
+    if tables.dim() != 2 or refs.dim() != 1:
+        raise ValueError("tables must be (requests, columns), refs (pages,)")
+    requests, columns = tables.shape
+    _ints("tables", tables, requests, columns)
+    _ints("lengths", lengths, requests)
+    _ints("refs", refs, refs.shape[0])
+    return PagedCacheDesc(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), requests, columns, refs.shape[0],
+                          page_size)
+
+
+def _head_rows(name: str, t: torch.Tensor) -> int:
+    """The row stride of (rows, heads, head_dim) bf16 values whose rows are whole, 16-byte aligned."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3:
+        raise ValueError(f"{name} must be (rows, heads, head_dim) bf16, got {t.dtype} {tuple(t.shape)}")
+    rows, heads, dim = t.shape
+    across, head, one = t.stride()
+    if rows <= 1:
+        across = heads * dim
+    if one != 1 or (head != dim and heads > 1) or across < heads * dim or across % 8 or t.is_neg():
+        raise ValueError(f"{name} must hold whole rows, a multiple of 8 values apart")
+    return across
+
+
+def _pages_shape(k_pages: torch.Tensor, v_pages: torch.Tensor) -> tuple[int, int, int, int]:
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+        raise ValueError("keys and values must be (pages, kv_heads, page_size, head_dim) of the same shape")
+    for t in (k_pages, v_pages):
+        if t.dtype is not torch.bfloat16 or not t.is_contiguous() or t.is_neg():
+            raise ValueError("pages must be contiguous bf16")
+    return k_pages.shape
+
+
+def paged_reserve(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, counts: torch.Tensor, page_size: int,
+                  starts: torch.Tensor, ends: torch.Tensor, status: torch.Tensor, positions: torch.Tensor,
+                  slots: torch.Tensor, copies: torch.Tensor, pool: torch.Tensor | None = None) -> None:
+    """Pages, rows and slots for the next counts[r] tokens of every request (imq_paged_reserve), on the
+    current stream: tables (requests, columns), lengths, counts, ends, status (requests,), starts
+    (requests + 1,), refs (pages,), positions and slots (rows,), copies (requests, 2), all int32 on
+    the current GPU.  `pool` (planes, pages, ...): where the pages lie, keys and values of every layer; pages that a
+    request stops sharing are copied in it.  status[r]: 0 taken, 1 no pages, 2 malformed, 3 no rows."""
+    desc = _cache_desc(tables, lengths, refs, page_size)
+    requests, rows = desc.requests, positions.shape[0] if positions.dim() == 1 else -1
+    _ints("counts", counts, requests)
+    _ints("starts", starts, requests + 1)
+    _ints("ends", ends, requests)
+    _ints("status", status, requests)
+    _ints("positions", positions, rows)
+    _ints("slots", slots, rows)
+    _ints("copies", copies, requests, 2)
+    _current_gpu(tables, lengths, refs, counts, starts, ends, status, positions, slots, copies)
+    planes = page_bytes = address = 0
+    if pool is not None:
+        if pool.dim() < 3 or pool.shape[1] != desc.pages or not pool.is_contiguous():
+            raise ValueError(f"the pool must be a contiguous (planes, {desc.pages}, ...) tensor")
+        _same_device(tables.get_device(), pool)
+        planes, page_bytes = pool.shape[0], pool.stride(1) * pool.element_size()
+        address = pool.data_ptr()
+    chunk = PagedChunkDesc(starts.data_ptr(), ends.data_ptr(), status.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+                           copies.data_ptr(), rows)
+    _check((_lib or lib()).imq_paged_reserve(ctypes.byref(desc), counts.data_ptr(), ctypes.byref(chunk), address, planes,
+                                             page_bytes, _stream(None)))
+
+
+def paged_reorder(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor,
+                  page_size: int) -> None:
+    """Request r becomes a copy of request parents[r], sharing its pages; -1: it becomes empty
+    (imq_paged_reorder), on the current stream.  Forks, beams' reordering, the end of requests."""
+    desc = _cache_desc(tables, lengths, refs, page_size)
+    _ints("parents", parents, desc.requests)
+    _current_gpu(tables, lengths, refs, parents)
+    _check((_lib or lib()).imq_paged_reorder(ctypes.byref(desc), parents.data_ptr(), _stream(None)))
+
+
+def paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
+                positions: torch.Tensor, slots: torch.Tensor, q_out: torch.Tensor, k_pages: torch.Tensor,
+                v_pages: torch.Tensor, theta: float, eps: float) -> torch.Tensor:
+    """Per-head RMSNorm and rotary embedding of q and k (imq_paged_write), on the current stream: q (rows, heads,
+    head_dim) to q_out, k and v (rows, kv_heads, head_dim) to the pages at `slots`; rows whose slot is
+    outside the pages are left out.  Rows may lie apart (a slice of a wider projection)."""
+    pages, kv_heads, page_size, dim = _pages_shape(k_pages, v_pages)
+    ldq, ldk, ldv, ldo = (_head_rows(*x) for x in (("q", q), ("k", k), ("v", v), ("q_out", q_out)))
+    rows, heads, _ = q.shape
+    if q.shape != q_out.shape or q.shape[2] != dim or k.shape != (rows, kv_heads, dim) or v.shape != k.shape:
+        raise ValueError("q and q_out must agree, k and v be (rows, kv_heads, head_dim) of the pages")
+    for w in (q_norm, k_norm):
+        if w.dtype is not torch.bfloat16 or w.shape != (dim,) or not w.is_contiguous():
+            raise ValueError(f"a norm weight must have {dim} bf16 values")
+    _ints("positions", positions, rows)
+    _ints("slots", slots, rows)
+    _current_gpu(q, k, v, q_norm, k_norm, positions, slots, q_out, k_pages, v_pages)
+    _check((_lib or lib()).imq_paged_write(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, q_norm.data_ptr(),
+                                           k_norm.data_ptr(), positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
+                                           ldo, k_pages.data_ptr(), v_pages.data_ptr(), rows, heads, kv_heads, dim, pages,
+                                           page_size, theta, eps, _stream(None)))
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, tables: torch.Tensor,
+                    starts: torch.Tensor, ends: torch.Tensor, out: torch.Tensor, scale: float, window: int = 0,
+                    max_context: int | None = None) -> torch.Tensor:
+    """Attention of every request's new tokens over its pages (imq_paged_attention), on the current
+    stream: q and out (rows, heads, head_dim) bf16, rows starts[r] .. starts[r + 1] - 1 of request r at its positions
+    up to ends[r] - 1, each over the positions up to its own (the last `window` of them).  max_context
+    (default: what the tables can hold) bounds `ends` and only plans the launch."""
+    pages, kv_heads, page_size, dim = _pages_shape(k_pages, v_pages)
+    ldq, ldo = _head_rows("q", q), _head_rows("out", out)
+    rows, heads, _ = q.shape
+    if q.shape != out.shape or q.shape[2] != dim:
+        raise ValueError(f"q and out must be (rows, heads, {dim})")
+    if tables.dim() != 2:
+        raise ValueError("tables must be (requests, columns)")
+    requests, columns = tables.shape
+    _ints("tables", tables, requests, columns)
+    _ints("starts", starts, requests + 1)
+    _ints("ends", ends, requests)
+    _current_gpu(q, k_pages, v_pages, tables, starts, ends, out)
+    library = _lib or lib()
+    context = columns * page_size if max_context is None else max_context
+    nbytes = library.imq_paged_attention_workspace(rows, requests, heads, kv_heads, dim, context, window)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _check(library.imq_paged_attention(q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(),
+                                       starts.data_ptr(), ends.data_ptr(), out.data_ptr(), ldo, rows, requests, columns,
+                                       pages, page_size, heads, kv_heads, dim, context, window, scale,
+                                       ws.data_ptr() if nbytes else None, nbytes, _stream(None)))
+    return out
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: int,
+                finished: torch.Tensor | None = None, eos: int = -1):
+    """The `count` best continuations of each group of `beams` beams (imq_beam_select), on the current
+    stream: logits (groups * beams, vocab) fp32 or bf16, scores (groups * beams,) fp32, finished int32
+    flags of beams that offer only themselves (token eos).  Returns (scores fp32, parents, tokens,
+    finished int32), each (groups, count), the best first; -inf, -1, -1, 0 where there are fewer."""
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or logits.is_neg():
+        raise ValueError("logits must be (beams, vocab) fp32 or bf16")
+    rows, vocab = logits.shape
+    ld = logits.stride(0) if rows > 1 else vocab
+    if (logits.stride(1) != 1 and vocab > 1) or ld < vocab:
+        raise ValueError("a row of logits must be whole")
+    if beams < 1 or rows < 1 or rows % beams:
+        raise ValueError(f"{rows} rows of logits are not groups of {beams} beams")
+    if scores.dtype is not torch.float32 or scores.shape != (rows,) or not scores.is_contiguous() or scores.is_neg():
+        raise ValueError(f"scores must be ({rows},) fp32")
+    _current_gpu(logits, scores)
+    if finished is not None:
+        _ints("finished", finished, rows)
+        _same_device(logits.get_device(), finished)
+    groups, library = rows // beams, _lib or lib()
+    nbytes = library.imq_beam_select_workspace(groups, beams, vocab, count)
+    if nbytes == 0:
+        raise NativeError(*last_error())
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device)
+    best = torch.empty((groups, count), dtype=torch.float32, device=logits.device)
+    made = torch.empty((3, groups, count), dtype=torch.int32, device=logits.device)
+    parents, tokens, ended = made.unbind(0)
+    _check(library.imq_beam_select(logits.data_ptr(), ld, _DTYPE_CODE[logits.dtype], scores.data_ptr(),
+                                   finished.data_ptr() if finished is not None else None, eos, groups, beams, vocab, count,
+                                   best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ended.data_ptr(),
+                                   ws.data_ptr(), nbytes, _stream(None)))
+    return best, parents, tokens, ended
 
 
 # --------------------------------------------------------------- decode-step kernels
