@@ -52,12 +52,15 @@ struct ReserveArgs {
   int32_t requests, columns, pages, shift, rows;
 };
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int u = __shfl_up(v, d);
-    if ((int)(threadIdx.x & 63) >= d) v += u;
-  }
+// Inclusive sum over the wavefront's lanes up to each: within each 16 by shifts, then lane 15 of a row
+// into the next one, then lane 31 into the upper half.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast 15, into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast 31, into rows 2 and 3
   return v;
 }
 
@@ -414,51 +417,104 @@ __global__ __launch_bounds__(kThreads) void write_kernel(const uint16_t* __restr
 // ------------------------------------------------------------ attention over pages
 //
 // The rows of a request and the query heads of one KV head are taken together as G n queries (row i,
-// head g of the group: query i G + g).  A wavefront takes a tile of 16 queries of one KV head and
-// walks the keys 32 at a time.  Scores are K Q^T on v_mfma_f32_16x16x32_bf16, so that a lane holds
-// keys of one query: P^T is then the B operand of V^T P^T without leaving its lane (keys 4 g .. of two
-// 16-key tiles).  K goes from its page to the A operand directly; V goes through LDS by rows and is
-// read transposed.
-typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
-
+// head g of the group: query i G + g), in tiles.  The work is shared out on the device, where the
+// lengths are: every workgroup adds up the key blocks of the requests' tiles and finds its own part.  Tiles
+// that several workgroups share leave fp32 partial results, which a second launch, by the same sums,
+// adds up in the order of their keys.
 struct AttendArgs {
   const uint16_t *q, *k_pages, *v_pages;
   const int32_t *tables, *starts, *ends;
   uint16_t* out;
   int64_t ldq, ldo;
+  float* partial;     // (slot, KV head, query of the tile, head_dim)
+  float2* state;      // (slot, KV head, query of the tile): the maximum (of scale_log2 q.k) and the sum
   int32_t rows, requests, columns, pages, shift, Hq, Hkv, group, window;
-  float scale_log2;  // scale * log2(e)
+  int32_t fewest, most;  // the queries n group of a request that this launch serves
+  int32_t units;      // parts to share the work out in, per KV head; there are 2 units slots
+  int32_t grain;      // log2 of the blocks that are counted as one (see attend_grain)
+  float scale_log2;   // scale * log2(e)
 };
 
-// The request whose tile `tile` is (tiles of `width` queries, requests in order), the tile's place in
-// it, its first row and its number of rows; false past the last tile.  The whole wavefront agrees.
-__device__ __forceinline__ bool find_tile(const AttendArgs& a, int tile, int width, int* request, int* place, int* first,
-                                          int* count) {
-  const int lane = threadIdx.x & 63;
-  int before = 0;
-  for (int base = 0; base < a.requests; base += 64) {
-    const int r = base + lane;
-    int lo = 0, n = 0;
-    if (r < a.requests) {
-      lo = clamp_int(a.starts[r], 0, a.rows);
-      n = clamp_int(a.starts[r + 1], lo, a.rows) - lo;
-    }
-    const int tiles = (n * a.group + width - 1) / width;
-    const int upto = before + wave_scan(tiles);
-    const uint64_t past = __ballot(upto > tile);
-    if (past) {
-      const int at = __ffsll((unsigned long long)past) - 1;
-      *request = base + at;
-      // (clamped: starts that do not ascend must not lead outside the request)
-      *place = clamp_int(tile - __builtin_amdgcn_readlane(upto - tiles, at), 0, __builtin_amdgcn_readlane(tiles, at) - 1);
-      *first = __builtin_amdgcn_readlane(lo, at);
-      *count = __builtin_amdgcn_readlane(n, at);
-      return true;
-    }
-    before = __builtin_amdgcn_readlane(upto, 63);
+// A request as the launch sees it: its first row and its rows, its tokens, its tiles of WIDTH queries,
+// the first block of BLOCK keys that any of them sees, and the blocks, in grains, from there to its end.
+struct Request {
+  int first, count, end, tiles, block0, blocks;
+};
+
+template <int WIDTH, int BLOCK>
+__device__ __forceinline__ Request read_request(const AttendArgs& a, int r) {
+  Request q = {0, 0, 0, 0, 0, 0};
+  if (r < a.requests) {
+    q.first = clamp_int(a.starts[r], 0, a.rows);
+    q.count = clamp_int(a.starts[r + 1], q.first, a.rows) - q.first;
+    q.end = clamp_int(a.ends[r], 0, a.columns << a.shift);
+    const int queries = q.count * a.group;
+    q.tiles = queries < a.fewest || queries > a.most ? 0 : (queries + WIDTH - 1) / WIDTH;
+    q.block0 = (a.window ? max(0, q.end - q.count - a.window + 1) : 0) / BLOCK;
+    q.blocks = max(1, (((q.end + BLOCK - 1) / BLOCK - q.block0) + (1 << a.grain) - 1) >> a.grain);
   }
-  return false;
+  return q;
 }
+
+// The request of lane `at`, in every lane.
+__device__ __forceinline__ Request from_lane(const Request& q, int at) {
+  return Request{__builtin_amdgcn_readlane(q.first, at), __builtin_amdgcn_readlane(q.count, at),
+                 __builtin_amdgcn_readlane(q.end, at),   __builtin_amdgcn_readlane(q.tiles, at),
+                 __builtin_amdgcn_readlane(q.block0, at), __builtin_amdgcn_readlane(q.blocks, at)};
+}
+
+// The requests' tiles one after another, each as long as `weight` says of its request: a line along which
+// the work of a KV head is shared out.  Every wavefront keeps the 64 requests it looked at last, one a lane.
+template <int WIDTH, int BLOCK, typename WEIGHT>
+struct Line {
+  const AttendArgs& a;
+  WEIGHT weight;
+  Request lane_request;
+  int upto;  // the line up to and with the lane's request
+  int base = 0, before = 0, total = 0;
+
+  __device__ __forceinline__ void read() {
+    lane_request = read_request<WIDTH, BLOCK>(a, base + (threadIdx.x & 63));
+    upto = before + wave_scan(lane_request.tiles * weight(lane_request));
+  }
+  __device__ __forceinline__ Line(const AttendArgs& args, WEIGHT w) : a(args), weight(w) {
+    for (;;) {
+      read();
+      total = __builtin_amdgcn_readlane(upto, 63);
+      if (base + 64 >= a.requests) break;
+      base += 64;
+      before = total;
+    }
+  }
+  // The request at point x of the line, its number and where it starts; false past the end.
+  __device__ __forceinline__ bool find(int x, Request* q, int* number, int* start) {
+    if (x < before || (x >= __builtin_amdgcn_readlane(upto, 63) && base + 64 < a.requests)) {
+      base = before = 0;
+      read();
+      while (x >= __builtin_amdgcn_readlane(upto, 63) && base + 64 < a.requests) {
+        before = __builtin_amdgcn_readlane(upto, 63);
+        base += 64;
+        read();
+      }
+    }
+    const uint64_t past = __ballot(upto > x);
+    if (!past) return false;
+    const int at = __ffsll((unsigned long long)past) - 1;
+    *q = from_lane(lane_request, at);
+    *number = base + at;
+    *start = __builtin_amdgcn_readlane(upto, at) - q->tiles * weight(*q);
+    return true;
+  }
+};
+
+struct BlocksOf {
+  __device__ __forceinline__ int operator()(const Request& q) const { return q.blocks; }
+};
+
+__device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // v_cvt_pk_bf16_f32
   bf16x2v r;
@@ -468,6 +524,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // v_cvt_pk
 }
 
 typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
+// (page numbers of a whole wavefront, which no kernel that reads them writes: loaded by the scalar unit)
+typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 
 // The bf16 pair `w` with infinities and NaNs as zeros; *odd gets a bit set if there were any.
 __device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t* odd) {
@@ -476,142 +534,706 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t* odd) {
   return (lo ? 0u : w & 0xffffu) | (hi ? 0u : w & 0xffff0000u);
 }
 
+// Few queries per request (decode steps, short chunks): tiles of 16 queries of one KV head.  The line of
+// blocks is cut into `units` equal parts whatever tiles they belong to, a workgroup takes one, tile
+// after tile, and each of its four wavefronts a quarter of a tile's keys there, 32 at a time.
+// Scores are K Q^T on v_mfma_f32_16x16x32_bf16, so that a lane holds keys of one query: P^T is then
+// the B operand of V^T P^T without leaving its lane (keys 4 g .. of two 16-key tiles).  K goes from
+// its page to the A operand directly; V goes through the wavefront's own LDS by rows, 32-byte pieces
+// swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
+// used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
+// over the softmax and P V, and no barrier before the wavefronts' results are joined.
+constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 4;
+constexpr int kRowsMost = 32;  // queries of a request that attend_rows_kernel is there for
 template <int D>
-__global__ __launch_bounds__(64) void attend_rows_kernel(AttendArgs a) {
+constexpr int kRowsWorkgroups = D == 128 ? 512 : 256;  // as many as are resident
+constexpr int kTileWorkgroups = 512;
+
+// The length of a part of the line.
+__device__ __forceinline__ int part_length(const AttendArgs& a, int total, int least) {
+  return max(least, (total + a.units - 1) / a.units);
+}
+
+template <int D>
+__device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& s, int request, int place, int from, int to,
+                                            int slot, char* lds, float (*tops)[16], float (*sums)[16]) {
   constexpr int T = D / 32, P = D / 8, C = D / 16;  // k-steps of a score, 16-byte pieces of a row, 16-dim tiles
-  __shared__ __attribute__((aligned(16))) char vl[32 * 2 * D];
-  const int head = blockIdx.x % a.Hkv, lane = threadIdx.x, n = lane & 15, g = lane >> 4;
-  int request, place, first, count;
-  if (!find_tile(a, blockIdx.x / a.Hkv, 16, &request, &place, &first, &count)) return;
-  const int end = clamp_int(a.ends[request], 0, a.columns << a.shift);
+  constexpr int V = 32 * P / 64;                    // 16-byte pieces of a block's values per lane
+  constexpr int kBytes = 32 * 2 * D;
+  const int head = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int query = 16 * place + n, row = query / a.group;
-  const bool live = row < count;
-  const int position = end - count + row;
-  const int tile_first = end - count + (16 * place) / a.group;
-  const int tile_last = min(end - 1, end - count + (16 * place + 15) / a.group);
+  const bool live = row < s.count;
+  const int begin = s.end - s.count;  // position of the request's first row
+  const int position = begin + row;
+  const int tile_first = begin + (16 * place) / a.group;
+  const int tile_last = min(s.end - 1, begin + (16 * place + 15) / a.group);
   const int low = a.window ? max(0, tile_first - a.window + 1) : 0;
   const int64_t q_head = (int64_t)head * a.group + query % a.group;
 
-  bf16x8_t qf[T];
-#pragma unroll
-  for (int t = 0; t < T; ++t) {
-    u32x4_t w = {0u, 0u, 0u, 0u};
-    if (live) w = *reinterpret_cast<const u32x4_t*>(a.q + (first + row) * a.ldq + q_head * D + 32 * t + 8 * g);
-    qf[t] = __builtin_bit_cast(bf16x8_t, w);
-  }
+  // the wavefront's blocks: its quarter of those between from and to that the tile sees
+  from = max(from, low / kRowsBlock);
+  to = tile_last < low ? from : min(to, tile_last / kRowsBlock + 1);
+  const int per_wave = (to - from + 3) >> 2;
+  int at = __builtin_amdgcn_readfirstlane(min(to, from + wave * per_wave));
+  const int stop = __builtin_amdgcn_readfirstlane(min(to, from + (wave + 1) * per_wave));
+
   f32x4_t o[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) o[c] = f32x4_t{};
   float top = -INFINITY, sum = 0.0f;
-  const int32_t* const table = a.tables + (int64_t)request * a.columns;
-  const int mask = (1 << a.shift) - 1;
 
-  for (int k0 = low & ~31; k0 <= tile_last; k0 += 32) {
-    // the two 16-key groups' pages (a page holds a multiple of 16 tokens)
-    int page[2];
-    bool held[2];
+  if (at < stop) {
+    bf16x8_t qf[T];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int key = k0 + 16 * b;
-      page[b] = key <= tile_last ? table[key >> a.shift] : -1;
-      held[b] = page[b] >= 0 && page[b] < a.pages;
-      page[b] = held[b] ? page[b] : 0;
-    }
-    f32x4_t s[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int64_t at = ((((int64_t)page[b] * a.Hkv + head) << a.shift) + ((k0 + 16 * b) & mask) + n) * D;
-      s[b] = f32x4_t{};
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(a.k_pages + at + 32 * t + 8 * g);
-        s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, w), qf[t], s[b], 0, 0, 0);
-      }
-    }
-    // V to LDS: rows that no query sees are zeros, whatever their page holds.  Where some queries see a
-    // key and others do not, a probability of zero must not meet an infinity or a NaN: such values
-    // are zeros in LDS, and are added below for the queries that see them.
-    const bool edge = k0 + 31 > tile_first || (a.window && k0 <= tile_last - a.window);
-    uint32_t odd = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 32 * P / 64; ++i) {
-      const int p = lane + 64 * i, r = p / P, b = r >> 4, key = k0 + r;
+    for (int t = 0; t < T; ++t) {
       u32x4_t w = {0u, 0u, 0u, 0u};
-      if (held[b] && key >= low && key <= tile_last)
-        w = *reinterpret_cast<const u32x4_t*>(a.v_pages + ((((int64_t)page[b] * a.Hkv + head) << a.shift) + (key & mask)) * D + 8 * (p % P));
+      if (live) w = *reinterpret_cast<const u32x4_t*>(a.q + (s.first + row) * a.ldq + q_head * D + 32 * t + 8 * g);
+      qf[t] = __builtin_bit_cast(bf16x8_t, w);
+    }
+    const scalar_ints table = (scalar_ints)(a.tables + (int64_t)request * a.columns);
+    const int mask = (1 << a.shift) - 1;
+    const uint32_t k_lane = 2 * (n * D + 8 * g), v_lane = 2 * ((lane / P) * D + 8 * (lane % P));
+    char* const vl = lds + wave * kBytes;
+
+    // the pages of a block's two 16-key groups (a page holds a multiple of 16 tokens)
+    struct Pair {
+      int page[2];
+    };
+    auto look_up = [&](int block) {
+      Pair p;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) p.page[b] = table[min(block * 32 + 16 * b, tile_last) >> a.shift];
+      return p;
+    };
+    auto held = [&](int page) { return (uint32_t)page < (uint32_t)a.pages; };
+    auto group_offset = [&](const Pair& p, int block, int b) {  // bytes; a bad page reads as page 0
+      const int page = held(p.page[b]) ? p.page[b] : 0;
+      return 2 * ((((int64_t)page * a.Hkv + head) << a.shift) + ((block * 32 + 16 * b) & mask)) * D;
+    };
+    u32x4_t kr[2][T], vr[V];
+    auto load_k = [&](const Pair& p, int block) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const char* const base = reinterpret_cast<const char*>(a.k_pages) + group_offset(p, block, b);
+#pragma unroll
+        for (int t = 0; t < T; ++t) kr[b][t] = *reinterpret_cast<const u32x4_t*>(base + k_lane + 64 * t);
+      }
+    };
+    auto load_v = [&](const Pair& p, int block) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const char* const base = reinterpret_cast<const char*>(a.v_pages) + group_offset(p, block, b);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i)
+          vr[b * (V / 2) + i] = *reinterpret_cast<const u32x4_t*>(base + v_lane + 1024 * i);
+      }
+    };
+    Pair now = look_up(at), next = look_up(min(at + 1, stop - 1));
+    load_k(now, at);
+    load_v(now, at);
+    for (; at < stop; ++at) {
+      const int ahead = min(at + 1, stop - 1), k0 = 32 * at;
+      f32x4_t sc[2];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        sc[b] = f32x4_t{};
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+          sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kr[b][t]), qf[t], sc[b], 0, 0, 0);
+      }
+      load_k(next, ahead);
+      // Where some queries see a key of the block and others do not, or none does: keys masked, values that
+      // nothing sees zeros whatever their page holds, and infinities and NaNs, which a probability of
+      // zero must not meet, zeros too; those are added below for the queries that see them.
+      const bool edge = k0 + 31 > tile_first || k0 < low || (a.window && k0 <= tile_last - a.window) ||
+                        !held(now.page[0]) || !held(now.page[1]);
+      uint32_t odd = 0;
       if (edge) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = finite_pair(w[e], &odd);
+        for (int i = 0; i < V; ++i) {
+          const int key = k0 + (64 / P) * i + lane / P;
+          const bool some = held(now.page[i / (V / 2)]) && key >= low && key <= tile_last;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vr[i][e] = some ? finite_pair(vr[i][e], &odd) : 0u;
+        }
       }
-      *reinterpret_cast<u32x4_t*>(vl + r * 2 * D + 16 * (p % P)) = w;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const int r = (64 / P) * i + lane / P, piece = lane % P;
+        *reinterpret_cast<u32x4_t*>(vl + r * 2 * D + 32 * ((piece >> 1) ^ (r & 7)) + 16 * (piece & 1)) = vr[i];
+      }
+      load_v(next, ahead);
+      const Pair after = look_up(min(at + 2, stop - 1));
+      float most = top;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[b][e] *= a.scale_log2;
+          if (edge) {
+            const int key = k0 + 16 * b + 4 * g + e;
+            if (!(held(now.page[b]) && key <= position && (!a.window || key > position - a.window))) sc[b][e] = -INFINITY;
+          }
+          most = fmaxf(most, sc[b][e]);  // (a NaN score comes back through its exponential)
+        }
+      most = max_xor32(max_xor16(most));
+      const float base = most == -INFINITY ? 0.0f : most;
+      const float keep = __builtin_amdgcn_exp2f(top - base);
+      top = most;
+      sum *= keep;
+      float p[2][4];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          p[b][e] = __builtin_amdgcn_exp2f(sc[b][e] - base);
+          sum += p[b][e];
+        }
+      const u32x4_t pw = {pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]),
+                          pack_bf16(p[1][2], p[1][3])};
+      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw);
+      __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        o[c] *= keep;
+        // lane i of each 16 reads 8 bytes of row i / 4; the transposed read gives it the four rows' value
+        // of dimension i
+        const int r = 4 * g + (n >> 2);
+        char* const v0 = vl + r * 2 * D + 32 * (c ^ (r & 7)) + 8 * (n & 3);
+        const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v0);
+        const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v0 + 16 * 2 * D));
+        const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[c], 0, 0, 0);
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (__any(odd)) {
+        for (int r = 0; r < 32; ++r) {
+          const int b = r >> 4, key = k0 + r;
+          if (!held(b ? now.page[1] : now.page[0]) || key < low || key > tile_last) continue;
+          const float mine = b ? ((r & 2) ? ((r & 1) ? p[1][3] : p[1][2]) : ((r & 1) ? p[1][1] : p[1][0]))
+                               : ((r & 2) ? ((r & 1) ? p[0][3] : p[0][2]) : ((r & 1) ? p[0][1] : p[0][0]));
+          const float pr = __shfl(mine, n + 16 * ((r >> 2) & 3));
+          const bool seen = live && key <= position && (!a.window || key > position - a.window);
+          const uint16_t* const v = a.v_pages + group_offset(now, at, b) / 2 + (r & 15) * D;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t bits = v[16 * c + 4 * g + e];
+              if (seen && (bits & 0x7f80u) == 0x7f80u) o[c][e] += pr * bf16_bits_to_f32(bits);
+            }
+        }
+      }
+      now = next;
+      next = after;
+    }
+    sum = add_xor32(add_xor16(sum));
+  }
+
+  // the four wavefronts' results joined: each by its distance from the common maximum
+  if (lane < 16) {
+    tops[wave][lane] = top;
+    sums[wave][lane] = sum;
+  }
+  __syncthreads();  // (and every wavefront is through with its values in LDS)
+  const float most = fmaxf(fmaxf(tops[0][n], tops[1][n]), fmaxf(tops[2][n], tops[3][n]));
+  const float scale = exp2f(top - (most == -INFINITY ? 0.0f : most));
+  float4* const joined = reinterpret_cast<float4*>(lds);  // (wavefront, tile of 16 dims, lane): 4 kBytes
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    joined[(wave * C + c) * 64 + lane] = make_float4(o[c][0] * scale, o[c][1] * scale, o[c][2] * scale, o[c][3] * scale);
+  __syncthreads();
+  float total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) total += sums[w][n] * exp2f(tops[w][n] - (most == -INFINITY ? 0.0f : most));
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const int64_t result = ((int64_t)slot * a.Hkv + head) * 16 + n;
+#pragma unroll
+  for (int i = 0; i < C / 4; ++i) {
+    const int c = wave + 4 * i;
+    float4 v = joined[c * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 u = joined[(w * C + c) * 64 + lane];
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    if (!live) continue;
+    if (slot < 0) {
+      const u32x2_t four = {pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv)};
+      *reinterpret_cast<u32x2_t*>(a.out + (s.first + row) * a.ldo + q_head * D + 16 * c + 4 * g) = four;
+    } else {
+      *reinterpret_cast<float4*>(a.partial + result * D + 16 * c + 4 * g) = v;
+    }
+  }
+  if (slot >= 0 && live && wave == 0 && g == 0) a.state[result] = make_float2(most, total);
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * 32 * 2 * D];
+  __shared__ float tops[4][16], sums[4][16];
+  const int unit = blockIdx.x / a.Hkv;
+  Line<kRowsTile, kRowsBlock, BlocksOf> line(a, BlocksOf());
+  const int part = part_length(a, line.total, kRowsLeast);
+  if ((int64_t)unit * part >= line.total) return;
+  const int x0 = unit * part, x1 = min(line.total, x0 + part);
+  for (int x = x0; x < x1;) {
+    Request q;
+    int request, start;
+    if (!line.find(x, &q, &request, &start)) return;
+    const int place = (x - start) / q.blocks, in = (x - start) % q.blocks;
+    if (x < start || place >= q.tiles) return;  // (sums that starts which do not ascend have wrapped)
+    const int length = min(q.blocks - in, x1 - x);
+    // a tile not whole here: the workgroup's first partial result, or its last
+    const int slot = length == q.blocks ? -1 : 2 * unit + (x != x0);
+    if (x != x0) __syncthreads();
+    attend_rows<D>(a, q, request, place, q.block0 + (in << a.grain), q.block0 + ((in + length) << a.grain), slot, lds, tops, sums);
+    x += length;
+  }
+}
+
+// The partial results of a tile added up in order.  A workgroup takes kMergeQueries queries of it, a group of D / 4 lanes
+// the partial results i, i + SG, ..: as many groups share a query as there are partial results for,
+// the others take other queries, four at a time.
+constexpr int kMergeQueries = 16;
+
+template <int WIDTH, int D, typename SLOT>
+__device__ __forceinline__ void merge_tile(const AttendArgs& a, const Request& s, int place, int head, int q0, int parts,
+                                           SLOT slot_of, float4 (*sums)[4][D / 4], float (*totals)[4]) {
+  constexpr int L = D / 4, NG = kThreads / L;
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  int share = 1;
+  while (share < NG && share < parts) share *= 2;
+  const int mine = group % share;
+  const int64_t step = (int64_t)a.Hkv * WIDTH;
+  for (int qb = 0; qb < kMergeQueries; qb += 4 * (NG / share)) {
+    const int first = WIDTH * place + q0 + qb;
+    if (first / a.group >= s.count) return;
+    const int q = q0 + qb + 4 * (group / share);  // and the three behind it
+    const bool some = q < q0 + kMergeQueries && (WIDTH * place + q) / a.group < s.count;
+    const int64_t at = (int64_t)head * WIDTH + q;
+    float most[4], total[4];
+    float4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      most[j] = -INFINITY;
+      total[j] = 0.0f;
+      v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    if (some) {
+      // (rows behind the request's last one have slots of their own that hold anything: not used)
+      for (int i = lane; i < parts; i += L)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], a.state[at + j + slot_of(i) * step].x);
+#pragma unroll
+      for (int d = 1; d < L; d <<= 1)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], __shfl_xor(most[j], d));
+#pragma unroll 2
+      for (int i = mine; i < parts; i += share) {
+        const int64_t from = at + slot_of(i) * step;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 st = a.state[from + j];
+          const float w = exp2f(st.x - (most[j] == -INFINITY ? 0.0f : most[j]));
+          const float4 u = *reinterpret_cast<const float4*>(a.partial + (from + j) * D + 4 * lane);
+          total[j] = fmaf(st.y, w, total[j]);
+          v[j].x = fmaf(u.x, w, v[j].x);
+          v[j].y = fmaf(u.y, w, v[j].y);
+          v[j].z = fmaf(u.z, w, v[j].z);
+          v[j].w = fmaf(u.w, w, v[j].w);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      sums[group][j][lane] = v[j];
+      if (lane == 0) totals[group][j] = total[j];
     }
     __syncthreads();
-    float most = top;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = k0 + 16 * b + 4 * g + e;
-        const bool seen = live && held[b] && key <= position && (!a.window || key > position - a.window);
-        s[b][e] = seen ? s[b][e] * a.scale_log2 : -INFINITY;
-        most = fmaxf(most, s[b][e]);  // (a NaN score comes back through its exponential)
+    // the groups that shared a query write one of the four each
+    if (some)
+      for (int j = mine; j < 4; j += share) {
+        const int query = WIDTH * place + q + j, row = query / a.group;
+        if (row >= s.count) break;
+        float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float t = 0.0f;
+        for (int k = 0; k < share; ++k) {
+          const float4 u = sums[group - mine + k][j][lane];
+          r.x += u.x, r.y += u.y, r.z += u.z, r.w += u.w;
+          t += totals[group - mine + k][j];
+        }
+        const float inv = t == 0.0f ? 0.0f : 1.0f / t;
+        const u32x2_t four = {pack_bf16(r.x * inv, r.y * inv), pack_bf16(r.z * inv, r.w * inv)};
+        *reinterpret_cast<u32x2_t*>(a.out + (s.first + row) * a.ldo + ((int64_t)head * a.group + query % a.group) * D + 4 * lane) = four;
       }
-    most = max_xor32(max_xor16(most));
-    const float base = most == -INFINITY ? 0.0f : most;
-    const float keep = exp2f(top - base);
-    top = most;
-    sum *= keep;
-    float p[2][4];
+    __syncthreads();
+  }
+}
+
+// For attend_rows_kernel: a workgroup per boundary between two parts of the line, at work where it is
+// the first inside its tile.
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
+  __shared__ float4 sums[kThreads / (D / 4)][4][D / 4];
+  __shared__ float totals[kThreads / (D / 4)][4];
+  const int head = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv + 1;
+  Line<kRowsTile, kRowsBlock, BlocksOf> line(a, BlocksOf());
+  const int part = part_length(a, line.total, kRowsLeast);
+  if ((int64_t)unit * part >= line.total) return;
+  Request q;
+  int request, start;
+  if (!line.find(unit * part, &q, &request, &start)) return;
+  const int place = (unit * part - start) / q.blocks, tile = start + place * q.blocks;
+  if (tile == unit * part || tile < (unit - 1) * part) return;
+  const int first = unit - 1, last = (tile + q.blocks - 1) / part;
+  if (unit * part < start || place >= q.tiles || last >= a.units) return;  // (as in attend_rows_kernel)
+  merge_tile<kRowsTile, D>(a, q, place, head, 0, last - first + 1,
+                           [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 && tile > first * part)); }, sums, totals);
+}
+
+// Many queries per request (chunks of prompts): tiles of 128 queries of one KV head, each of a workgroup's
+// four wavefronts 32 of them; the key blocks go through LDS, shared by the four
+// and twice there, the next block's loads in flight in registers over the current one's work and one
+// barrier per block.  Scores are K Q^T on v_mfma_f32_32x32x16_bf16 and P^T the B operand of V^T P^T without
+// leaving its lane, as above (keys 4 h .. and 8 + 4 h .. of 16).  The running maximum follows only when
+// a score passes it by 2^8: until then the probabilities are up to 256, which costs no accuracy, and the
+// sums need not be scaled again.  K lies in LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both
+// swizzled so that the rows that a read takes at a time lie in different banks (the 32-byte pieces of
+// attend_rows_kernel and K's by row & 7 had every read conflict once: half of the LDS cycles).
+//
+// A tile is cut into splits of at most `chunk` blocks, the chunk such that there are about kTileWorkgroups
+// of them.  Tiles of requests that have several splits come first, and a request's last tiles, the longest,
+// before its first ones.
+constexpr int kTile = 128, kTileLeast = 512;  // (keys)
+constexpr float kSlack = 8.0f;
+
+template <int D>
+constexpr int tile_block() {
+  return D == 128 ? 64 : 32;  // keys
+}
+
+struct TilePart {
+  Request q;
+  int request, place, split, splits, slot;  // splits: of the request's longest tile; slot: of the tile's first
+};
+
+template <int KEYS>
+struct SplitsOf {  // a request's splits of a tile: where there is one only, or more
+  int chunk, several;
+  __device__ __forceinline__ int operator()(const Request& q) const {
+    const int splits = ceil_of(q.blocks, chunk);
+    return (splits > 1) == several ? splits : 0;
+  }
+};
+
+// The blocks of a split.
+template <int KEYS>
+__device__ __forceinline__ int tile_chunk(const AttendArgs& a) {
+  Line<kTile, KEYS, BlocksOf> work(a, BlocksOf());
+  return max(max(1, (kTileLeast / KEYS) >> a.grain), ceil_of(work.total, a.units));
+}
+
+// Split number `unit`; false past the last one.
+template <int KEYS>
+__device__ __forceinline__ bool find_part(const AttendArgs& a, int unit, int chunk, TilePart* p) {
+  Line<kTile, KEYS, SplitsOf<KEYS>> split(a, SplitsOf<KEYS>{chunk, 1});
+  int start, in;
+  if (unit < split.total) {
+    if (!split.find(unit, &p->q, &p->request, &start)) return false;
+    p->splits = ceil_of(p->q.blocks, chunk);
+    in = (unit - start) / p->splits;
+    p->split = (unit - start) - in * p->splits;
+    p->slot = unit - p->split;
+  } else {
+    Line<kTile, KEYS, SplitsOf<KEYS>> whole(a, SplitsOf<KEYS>{chunk, 0});
+    if (!whole.find(unit - split.total, &p->q, &p->request, &start)) return false;
+    in = unit - split.total - start;
+    p->splits = 1;
+    p->split = p->slot = 0;
+  }
+  p->place = p->q.tiles - 1 - in;
+  // (sums that starts which do not ascend have wrapped must not lead outside the request or the workspace)
+  return p->place >= 0 && in >= 0 && (p->splits == 1 || (p->slot >= 0 && p->slot + p->splits <= 2 * a.units));
+}
+
+// A tile's blocks: from *first on, as many as are returned, of KEYS keys.
+template <int KEYS>
+__device__ __forceinline__ int tile_blocks(const AttendArgs& a, const Request& q, int place, int* tile_first, int* tile_last,
+                                           int* low, int* first) {
+  const int begin = q.end - q.count;
+  *tile_first = begin + (kTile * place) / a.group;
+  *tile_last = min(q.end - 1, begin + (kTile * place + kTile - 1) / a.group);
+  *low = a.window ? max(0, *tile_first - a.window + 1) : 0;
+  *first = *low / KEYS;
+  return *tile_last < *low ? 0 : *tile_last / KEYS + 1 - *first;
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_tile_kernel(AttendArgs a) {
+  constexpr int KEYS = tile_block<D>(), B = KEYS / 32, T = D / 16, C = D / 32, P = D / 8;
+  constexpr int MINE = KEYS / 4, L = MINE * P / 64;  // keys of a block that a wavefront loads, 1 KB at a time
+  constexpr int GROUPS = KEYS / 16;
+  // (arrays of their own: a read of one does not wait for the loads into another)
+  __shared__ __attribute__((aligned(16))) char k0l[KEYS * 2 * D], k1l[KEYS * 2 * D], v0l[KEYS * 2 * D], v1l[KEYS * 2 * D];
+  const int head = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  TilePart s;
+  const int chunk = tile_chunk<KEYS>(a);
+  if (!find_part<KEYS>(a, blockIdx.x / a.Hkv, chunk, &s)) return;
+  int tile_first, tile_last, low, block0;
+  const int all = tile_blocks<KEYS>(a, s.q, s.place, &tile_first, &tile_last, &low, &block0);
+  const int splits = max(1, ceil_of(ceil_of(all, 1 << a.grain), chunk));  // of this tile
+  if (s.split >= splits) return;
+  const int query = kTile * s.place + 32 * wave + n, row = query / a.group;
+  const bool live = row < s.q.count;
+  const int position = s.q.end - s.q.count + row;
+  const int64_t q_head = (int64_t)head * a.group + query % a.group;
+  const int per_split = ceil_of(all, splits);
+  const int from = __builtin_amdgcn_readfirstlane(block0 + min(all, s.split * per_split));
+  const int stop = __builtin_amdgcn_readfirstlane(block0 + min(all, (s.split + 1) * per_split));
+
+  f32x16_t o[C];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+  for (int c = 0; c < C; ++c) o[c] = f32x16_t{};
+  float top = -INFINITY, sum = 0.0f;  // (in units of raw scores times scale_log2)
+
+  if (from < stop) {
+    const scalar_ints table = (scalar_ints)(a.tables + (int64_t)s.request * a.columns);
+    const int mask = (1 << a.shift) - 1;
+    // Of a block: the page of this wavefront's keys (a bad one read as page 0), and which 16-key groups have a
+    // bad page.
+    auto look_up = [&](int block, int* page, uint32_t* bad) __attribute__((always_inline)) {
+      block = min(block, stop - 1);
+      *page = 0;
+      *bad = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        p[b][e] = exp2f(s[b][e] - base);
-        sum += p[b][e];
+      for (int b = 0; b < GROUPS; ++b) {
+        const int p = table[min(block * KEYS + 16 * b, tile_last) >> a.shift];
+        const bool held = (uint32_t)p < (uint32_t)a.pages;
+        *bad |= held ? 0u : 1u << b;
+        *page = held && wave * MINE / 16 == b ? p : *page;
       }
-    const u32x4_t pw = {pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]),
-                        pack_bf16(p[1][2], p[1][3])};
-    const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw);
+    };
+    // Memory -> LDS, 1 KB a load: lane l gets the 16 bytes at l.  The swizzle is in where the lane reads: of
+    // row r it takes the piece that belongs in its place.  A wavefront's MINE keys lie in one page.
+    uint32_t k_from[L], v_from[L];
 #pragma unroll
-    for (int c = 0; c < C; ++c) {
-      o[c] *= keep;
-      // lane i of each 16 reads 8 bytes of row i / 4; the transposed read gives it the four rows' value
-      // of dimension i
-      char* const from = vl + (4 * g + (n >> 2)) * 2 * D + 32 * c + 8 * (n & 3);
-      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)from);
-      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(from + 16 * 2 * D));
-      const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-      o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[c], 0, 0, 0);
+    for (int i = 0; i < L; ++i) {
+      const int in = (64 / P) * i + lane / P, r = wave * MINE + in, piece = lane % P;
+      k_from[i] = in * 2 * D + 16 * (piece ^ (r & 15));
+      v_from[i] = in * 2 * D + 64 * ((piece >> 2) ^ (r & 3)) + 16 * (piece & 3);
     }
-    if (__any(odd)) {
-      for (int r = 0; r < 32; ++r) {
-        const int b = r >> 4, key = k0 + r;
-        if (!held[b] || key < low || key > tile_last) continue;
-        const float mine = (r & 16) ? ((r & 2) ? ((r & 1) ? p[1][3] : p[1][2]) : ((r & 1) ? p[1][1] : p[1][0]))
-                                    : ((r & 2) ? ((r & 1) ? p[0][3] : p[0][2]) : ((r & 1) ? p[0][1] : p[0][0]));
-        const float pr = __shfl(mine, n + 16 * ((r >> 2) & 3));
-        const bool seen = live && key <= position && (!a.window || key > position - a.window);
-        const uint16_t* const from = a.v_pages + ((((int64_t)page[b] * a.Hkv + head) << a.shift) + (key & mask)) * D;
+    auto load = [&](const uint16_t* pages, int page, int block, const uint32_t* lane_from, char* to) __attribute__((always_inline)) {
+      block = min(block, stop - 1);
+      const int64_t at = ((((int64_t)page * a.Hkv + head) << a.shift) + ((block * KEYS + wave * MINE) & mask)) * D;
+      const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(pages + at, MINE * 2 * D);
 #pragma unroll
-        for (int c = 0; c < C; ++c)
+      for (int i = 0; i < L; ++i)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc, (__attribute__((address_space(3))) void*)(to + wave * MINE * 2 * D + 1024 * i), 16, lane_from[i], 0, 0, 0);
+    };
+    // Where some queries see a key of the block and others do not, or none does (see attend_rows)
+    auto is_edge = [&](int block, uint32_t bad) __attribute__((always_inline)) {
+      const int k0 = block * KEYS;
+      return bad || k0 + KEYS - 1 > tile_first || k0 < low || (a.window && k0 <= tile_last - a.window);
+    };
+    bf16x8_t qf[T];
+    const uint32_t k_lane = n * 2 * D + 16 * (h ^ (n & 15));
+    auto scores = [&](const char* kb, uint32_t at, int t, f32x16_t* sc) __attribute__((always_inline)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t v = from[16 * c + 4 * g + e];
-            if (seen && (v & 0x7f80u) == 0x7f80u) o[c][e] += pr * bf16_bits_to_f32(v);
+      for (int b = 0; b < B; ++b) {
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(kb + 32 * b * 2 * D + (at ^ (32 * t)));
+        sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, w), qf[t], t ? sc[b] : f32x16_t{}, 0, 0, 0);
+      }
+    };
+    // One block: its scores in sc, its values in vb; the next one's keys are in kb, and its scores
+    // replace this one's.  The keys after that go to k_free, the next values to v_free.
+    f32x16_t sc[B];
+    int page1, page2;                // the next block's page, and the one's after that
+    uint32_t bad0, bad1, bad2;       // this block's bad groups, and those of the two
+    auto turn = [&](int block, const char* kb, char* k_free, char* vb, char* v_free) __attribute__((always_inline)) {
+      // this wavefront's part of the next keys and of these values has landed; past the barrier every
+      // wavefront's has, and nobody reads the free arrays
+      wait_vmem();
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      load(a.k_pages, page2, block + 2, k_from, k_free);
+      load(a.v_pages, page1, block + 1, v_from, v_free);
+      const int k0 = KEYS * block;
+      const bool edge = is_edge(block, bad0);
+      int odd = 0;
+      if (edge) {
+        // (what only edges need is worked out here, not kept in registers over the loop)
+        int l = lane, p = position;
+        asm volatile("" : "+v"(l), "+v"(p));
+        uint32_t found = 0;
+#pragma unroll
+        for (int i = 0; i < L; ++i) {
+          const int r = wave * MINE + (64 / P) * i + l / P, key = k0 + r;
+          const bool good = !((bad0 >> (r >> 4)) & 1) && key >= low && key <= tile_last;
+          u32x4_t* const at = reinterpret_cast<u32x4_t*>(vb + wave * MINE * 2 * D + 1024 * i + 16 * l);
+          u32x4_t w = *at;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = good ? finite_pair(w[e], &found) : 0u;
+          *at = w;
+        }
+        odd = __syncthreads_or((int)found);
+        const int first = a.window ? p - a.window : -1;  // (the last key that the query no longer sees)
+#pragma unroll
+        for (int b = 0; b < B; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * (l >> 5) + (i & 3);
+            const bool seen = !((bad0 >> (2 * b + (i >> 3))) & 1) & (key <= p) & (key > first);
+            sc[b][i] = seen ? sc[b][i] : -INFINITY;
           }
       }
-    }
-  }
-  sum = add_xor32(add_xor16(sum));
-  if (!live) return;
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* const to = a.out + (first + row) * a.ldo + q_head * D;
+      float most = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const u32x2_t four = {pack_bf16(o[c][0] * inv, o[c][1] * inv), pack_bf16(o[c][2] * inv, o[c][3] * inv)};
-    *reinterpret_cast<u32x2_t*>(to + 16 * c + 4 * g) = four;
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, sc[b][i]);  // (a NaN score comes back through its exponential)
+      most = max_xor32(most) * a.scale_log2;
+      if (__any(most > top + kSlack)) {
+        const float higher = fmaxf(most, top), base = higher == -INFINITY ? 0.0f : higher;
+        const float keep = __builtin_amdgcn_exp2f(top - base);
+        top = higher;
+        sum *= keep;
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] *= keep;
+      }
+      const float base = top == -INFINITY ? 0.0f : top;
+      // the next block's scores, and between their MFMAs this one's probabilities
+      f32x16_t ahead[B];
+      uint32_t k_at = k_lane;
+      asm volatile("" : "+v"(k_at));  // (one register, and an instruction for each read's address)
+      u32x4_t pw[KEYS / 16];
+#pragma unroll
+      for (int t = 0; t < T; ++t) scores(kb, k_at, t, ahead);
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sc[b][i] = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.scale_log2, -base));
+          sum += sc[b][i];
+        }
+#pragma unroll
+      for (int u = 0; u < KEYS / 16; ++u) {
+        const int b = u >> 1, i0 = 8 * (u & 1);
+        pw[u] = u32x4_t{pack_bf16(sc[b][i0], sc[b][i0 + 1]), pack_bf16(sc[b][i0 + 2], sc[b][i0 + 3]),
+                        pack_bf16(sc[b][i0 + 4], sc[b][i0 + 5]), pack_bf16(sc[b][i0 + 6], sc[b][i0 + 7])};
+      }
+      if (odd) {
+        int l = lane, p = live ? position : -1;
+        asm volatile("" : "+v"(l), "+v"(p));
+        for (int r = 0; r < KEYS; ++r) {
+          const int key = k0 + r;
+          if (((bad0 >> (r >> 4)) & 1) || key < low || key > tile_last) continue;
+          const int which = 16 * (r >> 5) + 4 * ((r >> 3) & 3) + (r & 3);
+          float mine = 0.0f;
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mine = which == 16 * b + i ? sc[b][i] : mine;
+          const float pr = __shfl(mine, (l & 31) + 32 * ((r >> 2) & 1));
+          const bool seen = key <= p && (!a.window || key > p - a.window);
+          const uint16_t* const v = a.v_pages + ((((int64_t)table[key >> a.shift] * a.Hkv + head) << a.shift) + (key & mask)) * D;
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t bits = v[32 * c + 8 * (i >> 2) + 4 * (l >> 5) + (i & 3)];
+              if (seen && (bits & 0x7f80u) == 0x7f80u) o[c][i] += pr * bf16_bits_to_f32(bits);
+            }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < KEYS / 16; ++u) {
+        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw[u]);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const int r = 16 * u + 4 * h + ((lane & 15) >> 2);
+          const char* const at = vb + r * 2 * D + 64 * (c ^ (r & 3)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+          const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+          const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * 2 * D));
+          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[c], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < B; ++b) sc[b] = ahead[b];
+      page1 = page2;
+      bad0 = bad1;
+      bad1 = bad2;
+      look_up(block + 3, &page2, &bad2);
+    };
+
+    int page0;
+    look_up(from, &page0, &bad0);
+    look_up(from + 1, &page1, &bad1);
+    look_up(from + 2, &page2, &bad2);
+    load(a.k_pages, page0, from, k_from, k0l);
+    load(a.k_pages, page1, from + 1, k_from, k1l);
+    load(a.v_pages, page0, from, v_from, v0l);
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      u32x4_t w = {0u, 0u, 0u, 0u};
+      if (live) w = *reinterpret_cast<const u32x4_t*>(a.q + (s.q.first + row) * a.ldq + q_head * D + 16 * t + 8 * h);
+      qf[t] = __builtin_bit_cast(bf16x8_t, w);
+    }
+    wait_vmem();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < T; ++t) scores(k0l, k_lane, t, sc);
+    for (int block = from; block < stop; block += 2) {
+      turn(block, k1l, k0l, v0l, v1l);
+      if (block + 1 < stop) turn(block + 1, k0l, k1l, v1l, v0l);
+    }
+    wait_vmem();  // the loads past the last block, before the LDS is given up
+    sum = add_xor32(sum);
   }
+  if (!live) return;
+  if (splits == 1) {
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint16_t* const to = a.out + (s.q.first + row) * a.ldo + q_head * D + 4 * h;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const u32x2_t four = {pack_bf16(o[c][i] * inv, o[c][i + 1] * inv), pack_bf16(o[c][i + 2] * inv, o[c][i + 3] * inv)};
+        *reinterpret_cast<u32x2_t*>(to + 32 * c + 2 * i) = four;
+      }
+    return;
+  }
+  const int64_t result = ((int64_t)(s.slot + s.split) * a.Hkv + head) * kTile + 32 * wave + n;
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<float4*>(a.partial + result * D + 32 * c + 2 * i + 4 * h) =
+          make_float4(o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]);
+  if (h == 0) a.state[result] = make_float2(top, sum);
+}
+
+// For attend_tile_kernel: a workgroup per 16 queries of a tile, at work where the unit is a tile's first split.
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_tile_kernel(AttendArgs a) {
+  __shared__ float4 sums[kThreads / (D / 4)][4][D / 4];
+  __shared__ float totals[kThreads / (D / 4)][4];
+  constexpr int KEYS = tile_block<D>();
+  const int head = blockIdx.x % a.Hkv;
+  const int chunk = tile_chunk<KEYS>(a);
+  TilePart s;
+  if (!find_part<KEYS>(a, blockIdx.x / a.Hkv, chunk, &s) || s.split || s.splits == 1) return;
+  int tile_first, tile_last, low, block0;
+  const int all = tile_blocks<KEYS>(a, s.q, s.place, &tile_first, &tile_last, &low, &block0);
+  const int splits = ceil_of(ceil_of(all, 1 << a.grain), chunk);
+  if (splits <= 1) return;
+  const int64_t slot = s.slot;
+  merge_tile<kTile, D>(a, s.q, s.place, head, kMergeQueries * blockIdx.y, splits, [&](int i) { return slot + i; }, sums, totals);
 }
 
 // ------------------------------------------------------------ host side
@@ -658,6 +1280,74 @@ int32_t check_heads(int32_t rows, int32_t Hq, int32_t Hkv, int32_t head_dim) {
   if (Hq > IMQ_PAGED_MAX_HEADS) return fail(IMQ_EUNSUPPORTED, "too many heads");
   if (head_dim != 128 && head_dim != 256) return fail(IMQ_EUNSUPPORTED, "the head size must be 128 or 256");
   return IMQ_OK;
+}
+
+// A launch for the requests with `fewest` to `most` queries of a KV head (`width` 0: none): the parts it
+// shares their work out in, per KV head, and the tiles there may be.
+struct AttendLaunch {
+  int64_t units, tiles;
+  int32_t fewest, most, width;
+};
+
+struct AttendPlan {
+  AttendLaunch few, many;
+};
+
+// Requests of up to kRowsMost queries go to attend_rows_kernel, longer ones to attend_tile_kernel.  The
+// host knows the sums only: where the average request stays within kRowsMost the first serves all.
+AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim) {
+  const int64_t queries = (int64_t)rows * (Hq / Hkv), with = std::min(rows, requests);
+  // at most one part-full tile for each request with rows
+  auto launch = [&](int workgroups, int width, int64_t fewest, int64_t most) {
+    return AttendLaunch{ceil_div(workgroups, Hkv), with + queries / width, (int32_t)fewest, (int32_t)most, width};
+  };
+  AttendPlan p;
+  memset(&p, 0, sizeof(p));
+  const bool all_few = queries <= kRowsMost * with, some_few = requests > 1;
+  if (all_few || some_few) p.few = launch(head_dim == 128 ? kRowsWorkgroups<128> : kRowsWorkgroups<256>, kRowsTile, 0, all_few ? INT32_MAX : kRowsMost);
+  if (!all_few) p.many = launch(kTileWorkgroups, kTile, some_few ? kRowsMost + 1 : 0, INT32_MAX);
+  return p;
+}
+
+// The partial results' part of a launch's workspace, then their maxima and sums.
+size_t attend_space(const AttendLaunch& l, int32_t Hkv, int32_t head_dim) {
+  return (size_t)l.units * 2 * Hkv * l.width * (head_dim * 4 + 8);
+}
+
+// log2 of the blocks that the device counts as one: 0 unless the sums of the blocks of all tiles could pass 30 bits.
+int attend_grain(const AttendLaunch& l, int64_t max_tokens) {
+  const double most = (double)l.tiles * (double)(max_tokens / 32 + 1);
+  int grain = 0;
+  while (most / (double)(1ll << grain) >= (double)(1 << 30)) ++grain;
+  return grain;
+}
+
+// A launch's fields of the arguments, its part of the workspace starting at `space`.
+AttendArgs with_launch(AttendArgs a, const AttendLaunch& l, int head_dim, char* space) {
+  a.fewest = l.fewest;
+  a.most = l.most;
+  a.units = (int32_t)l.units;
+  a.grain = attend_grain(l, (int64_t)a.columns << a.shift);
+  a.partial = reinterpret_cast<float*>(space);
+  a.state = reinterpret_cast<float2*>(a.partial + (size_t)l.units * 2 * a.Hkv * l.width * head_dim);
+  return a;
+}
+
+template <int D>
+void launch_attend(const AttendPlan& p, char* space, const AttendArgs& args, hipStream_t stream) {
+  if (p.few.width) {
+    const AttendArgs a = with_launch(args, p.few, D, space);
+    const dim3 grid((uint32_t)(p.few.units * a.Hkv));
+    hipLaunchKernelGGL(attend_rows_kernel<D>, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(merge_rows_kernel<D>, grid, dim3(kThreads), 0, stream, a);
+  }
+  if (p.many.width) {
+    const AttendArgs a = with_launch(args, p.many, D, space + attend_space(p.few, args.Hkv, D));
+    // at most 2 units of the splits of tiles of several, and a workgroup for every other tile
+    const int64_t split = 2 * p.many.units;
+    hipLaunchKernelGGL(attend_tile_kernel<D>, dim3((uint32_t)((split + p.many.tiles) * a.Hkv)), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(merge_tile_kernel<D>, dim3((uint32_t)(split * a.Hkv), kTile / kMergeQueries), dim3(kThreads), 0, stream, a);
+  }
 }
 
 bool row_stride(int64_t ld, int64_t width) { return ld >= width && ld % 8 == 0; }
@@ -741,7 +1431,9 @@ int32_t imq_paged_write(const uint16_t* q, int64_t ldq, const uint16_t* k, int64
 
 size_t imq_paged_attention_workspace(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim,
                                      int32_t max_context, int32_t window) {
-  return 0;
+  if (check_heads(rows, Hq, Hkv, head_dim) != IMQ_OK || rows == 0 || requests < 1) return 0;
+  const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim);
+  return attend_space(plan.few, Hkv, head_dim) + attend_space(plan.many, Hkv, head_dim);
 }
 
 int32_t imq_paged_attention(const uint16_t* q, int64_t ldq, const uint16_t* k_pages, const uint16_t* v_pages,
@@ -763,13 +1455,17 @@ int32_t imq_paged_attention(const uint16_t* q, int64_t ldq, const uint16_t* k_pa
   for (const void* p : {(const void*)q, (const void*)k_pages, (const void*)v_pages, (const void*)out})
     if (!p || !aligned(p, 16)) return fail(IMQ_EINVAL, "rows and pages must be non-null and 16-byte aligned");
   if (!current_device(&code)) return code;
-  const int group = Hq / Hkv;
-  AttendArgs a{q, k_pages, v_pages, tables, starts, ends, out, ldq, ldo, rows, requests, columns, pages,
-               __builtin_ctz(page_size), Hq, Hkv, group, window, scale * 1.44269504088896340736f};
-  // tiles of 16 queries: at most one part-full one for each request with rows
-  const int64_t tiles = std::min<int64_t>(rows, requests) + (int64_t)rows * group / 16;
-  const auto kernel = head_dim == 128 ? attend_rows_kernel<128> : attend_rows_kernel<256>;
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)(tiles * Hkv)), dim3(64), 0, static_cast<hipStream_t>(stream), a);
+  const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim);
+  if (!workspace || !aligned(workspace, 16) ||
+      workspace_bytes < attend_space(plan.few, Hkv, head_dim) + attend_space(plan.many, Hkv, head_dim))
+    return fail(IMQ_EINVAL, "the workspace is too small or not 16-byte aligned");
+  AttendArgs a{q, k_pages, v_pages, tables, starts, ends, out, ldq, ldo, nullptr, nullptr, rows, requests, columns, pages,
+               __builtin_ctz(page_size), Hq, Hkv, Hq / Hkv, window, 0, 0, 0, 0, scale * 1.44269504088896340736f};
+  char* const space = static_cast<char*>(workspace);
+  if (head_dim == 128)
+    launch_attend<128>(plan, space, a, static_cast<hipStream_t>(stream));
+  else
+    launch_attend<256>(plan, space, a, static_cast<hipStream_t>(stream));
   return launched("paged attention");
 }
 
