@@ -102,8 +102,10 @@ IMQ_API int32_t imq_paged_write(const uint16_t* q, int64_t ldq, const uint16_t* 
  * Rows outside every request are left as they were; a row that sees nothing gets zeros.  Keys in a
  * table entry outside 0 .. pages - 1 are left out.  Entries past a row's position are never used,
  * whatever they hold.  Starts ascend; values outside 0 .. rows are taken as the nearest bound.
- * `workspace`: imq_paged_attention_workspace bytes (may be 0), 16-byte aligned, no preparation; calls
- * that share one must not overlap.
+ * max_context: a bound on `ends` by which the launch is planned (the results do not depend on it
+ * beyond the order of sums; the tables' capacity will do).  `workspace`: imq_paged_attention_workspace
+ * bytes (may be 0) for the same max_context, 16-byte aligned, no preparation; calls that share one must not
+ * overlap.
  * The paged, many-row form of imq_attention_decode (ironmule/dense_plan.py:258-274). */
 IMQ_API size_t imq_paged_attention_workspace(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim,
                                              int32_t max_context, int32_t window);

@@ -430,7 +430,8 @@ struct AttendArgs {
   float2* state;      // (slot, KV head, query of the tile): the maximum (of scale_log2 q.k) and the sum
   int32_t rows, requests, columns, pages, shift, Hq, Hkv, group, window;
   int32_t fewest, most;  // the queries n group of a request that this launch serves
-  int32_t units;      // parts to share the work out in, per KV head; there are 2 units slots
+  int32_t units;      // parts to share the work out in, per KV head
+  int32_t slots;      // partial results there is room for, per KV head
   int32_t grain;      // log2 of the blocks that are counted as one (see attend_grain)
   float scale_log2;   // scale * log2(e)
 };
@@ -463,45 +464,57 @@ __device__ __forceinline__ Request from_lane(const Request& q, int at) {
                  __builtin_amdgcn_readlane(q.block0, at), __builtin_amdgcn_readlane(q.blocks, at)};
 }
 
-// The requests' tiles one after another, each as long as `weight` says of its request: a line along which
-// the work of a KV head is shared out.  Every wavefront keeps the 64 requests it looked at last, one a lane.
-template <int WIDTH, int BLOCK, typename WEIGHT>
-struct Line {
+// The 64 requests that a wavefront looked at last, one a lane.
+template <int WIDTH, int BLOCK>
+struct Lanes {
   const AttendArgs& a;
-  WEIGHT weight;
-  Request lane_request;
-  int upto;  // the line up to and with the lane's request
-  int base = 0, before = 0, total = 0;
-
-  __device__ __forceinline__ void read() {
-    lane_request = read_request<WIDTH, BLOCK>(a, base + (threadIdx.x & 63));
-    upto = before + wave_scan(lane_request.tiles * weight(lane_request));
+  Request q;
+  int base;
+  __device__ __forceinline__ explicit Lanes(const AttendArgs& args) : a(args), base(-1) {}
+  __device__ __forceinline__ void read(int from) {
+    if (from == base) return;
+    base = from;
+    q = read_request<WIDTH, BLOCK>(a, from + (threadIdx.x & 63));
   }
-  __device__ __forceinline__ Line(const AttendArgs& args, WEIGHT w) : a(args), weight(w) {
-    for (;;) {
-      read();
-      total = __builtin_amdgcn_readlane(upto, 63);
-      if (base + 64 >= a.requests) break;
-      base += 64;
+};
+
+// The requests' tiles one after another, each as long as `weight` says of its request: a line along which
+// the work of a KV head is shared out.
+template <typename LANES, typename WEIGHT>
+struct Line {
+  LANES& lanes;
+  WEIGHT weight;
+  int upto;  // the line up to and with the lane's request
+  int before = 0, total = 0;
+
+  __device__ __forceinline__ void read(int base) {
+    lanes.read(base);
+    upto = before + wave_scan(lanes.q.tiles * weight(lanes.q));
+  }
+  __device__ __forceinline__ Line(LANES& l, WEIGHT w) : lanes(l), weight(w) {
+    for (int base = 0;; base += 64) {
       before = total;
+      read(base);
+      total = __builtin_amdgcn_readlane(upto, 63);
+      if (base + 64 >= lanes.a.requests) break;
     }
   }
-  // The request at point x of the line, its number and where it starts; false past the end.
+  // The request at point x of the line: its number and where it starts; false past the end.
   __device__ __forceinline__ bool find(int x, Request* q, int* number, int* start) {
-    if (x < before || (x >= __builtin_amdgcn_readlane(upto, 63) && base + 64 < a.requests)) {
-      base = before = 0;
-      read();
-      while (x >= __builtin_amdgcn_readlane(upto, 63) && base + 64 < a.requests) {
+    const int requests = lanes.a.requests;
+    if (requests > 64) {  // (another line may have moved the lanes on)
+      before = 0;
+      read(0);
+      for (int base = 64; x >= __builtin_amdgcn_readlane(upto, 63) && base < requests; base += 64) {
         before = __builtin_amdgcn_readlane(upto, 63);
-        base += 64;
-        read();
+        read(base);
       }
     }
     const uint64_t past = __ballot(upto > x);
     if (!past) return false;
     const int at = __ffsll((unsigned long long)past) - 1;
-    *q = from_lane(lane_request, at);
-    *number = base + at;
+    *q = from_lane(lanes.q, at);
+    *number = lanes.base + at;
     *start = __builtin_amdgcn_readlane(upto, at) - q->tiles * weight(*q);
     return true;
   }
@@ -596,42 +609,37 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
     const uint32_t k_lane = 2 * (n * D + 8 * g), v_lane = 2 * ((lane / P) * D + 8 * (lane % P));
     char* const vl = lds + wave * kBytes;
 
-    // the pages of a block's two 16-key groups (a page holds a multiple of 16 tokens)
-    struct Pair {
-      int page[2];
-    };
-    auto look_up = [&](int block) {
-      Pair p;
-#pragma unroll
-      for (int b = 0; b < 2; ++b) p.page[b] = table[min(block * 32 + 16 * b, tile_last) >> a.shift];
-      return p;
-    };
+    // the pages of a block's two 16-key groups (a page holds a multiple of 16 tokens).  (Plain numbers, no
+    // array: as one they went to LDS, for whose layout the compiler has every workgroup read the launch's
+    // packet in host memory, one after another: 15 us for 256 of them.)
+    auto page_of = [&](int block, int b) { return table[min(block * 32 + 16 * b, tile_last) >> a.shift]; };
     auto held = [&](int page) { return (uint32_t)page < (uint32_t)a.pages; };
-    auto group_offset = [&](const Pair& p, int block, int b) {  // bytes; a bad page reads as page 0
-      const int page = held(p.page[b]) ? p.page[b] : 0;
+    auto group_offset = [&](int page, int block, int b) {  // bytes; a bad page reads as page 0
+      page = held(page) ? page : 0;
       return 2 * ((((int64_t)page * a.Hkv + head) << a.shift) + ((block * 32 + 16 * b) & mask)) * D;
     };
     u32x4_t kr[2][T], vr[V];
-    auto load_k = [&](const Pair& p, int block) {
+    auto load_k = [&](int page0, int page1, int block) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const char* const base = reinterpret_cast<const char*>(a.k_pages) + group_offset(p, block, b);
+        const char* const base = reinterpret_cast<const char*>(a.k_pages) + group_offset(b ? page1 : page0, block, b);
 #pragma unroll
         for (int t = 0; t < T; ++t) kr[b][t] = *reinterpret_cast<const u32x4_t*>(base + k_lane + 64 * t);
       }
     };
-    auto load_v = [&](const Pair& p, int block) {
+    auto load_v = [&](int page0, int page1, int block) {
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
-        const char* const base = reinterpret_cast<const char*>(a.v_pages) + group_offset(p, block, b);
+        const char* const base = reinterpret_cast<const char*>(a.v_pages) + group_offset(b ? page1 : page0, block, b);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
           vr[b * (V / 2) + i] = *reinterpret_cast<const u32x4_t*>(base + v_lane + 1024 * i);
       }
     };
-    Pair now = look_up(at), next = look_up(min(at + 1, stop - 1));
-    load_k(now, at);
-    load_v(now, at);
+    int now0 = page_of(at, 0), now1 = page_of(at, 1);
+    int next0 = page_of(min(at + 1, stop - 1), 0), next1 = page_of(min(at + 1, stop - 1), 1);
+    load_k(now0, now1, at);
+    load_v(now0, now1, at);
     for (; at < stop; ++at) {
       const int ahead = min(at + 1, stop - 1), k0 = 32 * at;
       f32x4_t sc[2];
@@ -642,18 +650,18 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
         for (int t = 0; t < T; ++t)
           sc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kr[b][t]), qf[t], sc[b], 0, 0, 0);
       }
-      load_k(next, ahead);
+      load_k(next0, next1, ahead);
       // Where some queries see a key of the block and others do not, or none does: keys masked, values that
       // nothing sees zeros whatever their page holds, and infinities and NaNs, which a probability of
       // zero must not meet, zeros too; those are added below for the queries that see them.
       const bool edge = k0 + 31 > tile_first || k0 < low || (a.window && k0 <= tile_last - a.window) ||
-                        !held(now.page[0]) || !held(now.page[1]);
+                        !held(now0) || !held(now1);
       uint32_t odd = 0;
       if (edge) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const int key = k0 + (64 / P) * i + lane / P;
-          const bool some = held(now.page[i / (V / 2)]) && key >= low && key <= tile_last;
+          const bool some = held(i / (V / 2) ? now1 : now0) && key >= low && key <= tile_last;
 #pragma unroll
           for (int e = 0; e < 4; ++e) vr[i][e] = some ? finite_pair(vr[i][e], &odd) : 0u;
         }
@@ -663,8 +671,8 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
         const int r = (64 / P) * i + lane / P, piece = lane % P;
         *reinterpret_cast<u32x4_t*>(vl + r * 2 * D + 32 * ((piece >> 1) ^ (r & 7)) + 16 * (piece & 1)) = vr[i];
       }
-      load_v(next, ahead);
-      const Pair after = look_up(min(at + 2, stop - 1));
+      load_v(next0, next1, ahead);
+      const int after0 = page_of(min(at + 2, stop - 1), 0), after1 = page_of(min(at + 2, stop - 1), 1);
       float most = top;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -673,7 +681,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
           sc[b][e] *= a.scale_log2;
           if (edge) {
             const int key = k0 + 16 * b + 4 * g + e;
-            if (!(held(now.page[b]) && key <= position && (!a.window || key > position - a.window))) sc[b][e] = -INFINITY;
+            if (!(held(b ? now1 : now0) && key <= position && (!a.window || key > position - a.window))) sc[b][e] = -INFINITY;
           }
           most = fmaxf(most, sc[b][e]);  // (a NaN score comes back through its exponential)
         }
@@ -710,12 +718,12 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
       if (__any(odd)) {
         for (int r = 0; r < 32; ++r) {
           const int b = r >> 4, key = k0 + r;
-          if (!held(b ? now.page[1] : now.page[0]) || key < low || key > tile_last) continue;
+          if (!held(b ? now1 : now0) || key < low || key > tile_last) continue;
           const float mine = b ? ((r & 2) ? ((r & 1) ? p[1][3] : p[1][2]) : ((r & 1) ? p[1][1] : p[1][0]))
                                : ((r & 2) ? ((r & 1) ? p[0][3] : p[0][2]) : ((r & 1) ? p[0][1] : p[0][0]));
           const float pr = __shfl(mine, n + 16 * ((r >> 2) & 3));
           const bool seen = live && key <= position && (!a.window || key > position - a.window);
-          const uint16_t* const v = a.v_pages + group_offset(now, at, b) / 2 + (r & 15) * D;
+          const uint16_t* const v = a.v_pages + group_offset(b ? now1 : now0, at, b) / 2 + (r & 15) * D;
 #pragma unroll
           for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -725,8 +733,8 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
             }
         }
       }
-      now = next;
-      next = after;
+      now0 = next0, now1 = next1;
+      next0 = after0, next1 = after1;
     }
     sum = add_xor32(add_xor16(sum));
   }
@@ -774,7 +782,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_rows_kernel
   __shared__ __attribute__((aligned(16))) char lds[4 * 32 * 2 * D];
   __shared__ float tops[4][16], sums[4][16];
   const int unit = blockIdx.x / a.Hkv;
-  Line<kRowsTile, kRowsBlock, BlocksOf> line(a, BlocksOf());
+  Lanes<kRowsTile, kRowsBlock> lanes(a);
+  Line<Lanes<kRowsTile, kRowsBlock>, BlocksOf> line(lanes, BlocksOf());
   const int part = part_length(a, line.total, kRowsLeast);
   if ((int64_t)unit * part >= line.total) return;
   const int x0 = unit * part, x1 = min(line.total, x0 + part);
@@ -879,7 +888,8 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
   __shared__ float4 sums[kThreads / (D / 4)][4][D / 4];
   __shared__ float totals[kThreads / (D / 4)][4];
   const int head = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv + 1;
-  Line<kRowsTile, kRowsBlock, BlocksOf> line(a, BlocksOf());
+  Lanes<kRowsTile, kRowsBlock> lanes(a);
+  Line<Lanes<kRowsTile, kRowsBlock>, BlocksOf> line(lanes, BlocksOf());
   const int part = part_length(a, line.total, kRowsLeast);
   if ((int64_t)unit * part >= line.total) return;
   Request q;
@@ -919,7 +929,6 @@ struct TilePart {
   int request, place, split, splits, slot;  // splits: of the request's longest tile; slot: of the tile's first
 };
 
-template <int KEYS>
 struct SplitsOf {  // a request's splits of a tile: where there is one only, or more
   int chunk, several;
   __device__ __forceinline__ int operator()(const Request& q) const {
@@ -929,33 +938,39 @@ struct SplitsOf {  // a request's splits of a tile: where there is one only, or 
 };
 
 // The blocks of a split.
-template <int KEYS>
-__device__ __forceinline__ int tile_chunk(const AttendArgs& a) {
-  Line<kTile, KEYS, BlocksOf> work(a, BlocksOf());
-  return max(max(1, (kTileLeast / KEYS) >> a.grain), ceil_of(work.total, a.units));
+template <typename LANES>
+__device__ __forceinline__ int tile_chunk(LANES& lanes, int least) {
+  const AttendArgs& a = lanes.a;
+  if (a.units == 0) return 1 << 30;
+  Line<LANES, BlocksOf> work(lanes, BlocksOf());
+  return max(max(1, least >> a.grain), ceil_of(work.total, a.units));
 }
 
-// Split number `unit`; false past the last one.
-template <int KEYS>
-__device__ __forceinline__ bool find_part(const AttendArgs& a, int unit, int chunk, TilePart* p) {
-  Line<kTile, KEYS, SplitsOf<KEYS>> split(a, SplitsOf<KEYS>{chunk, 1});
-  int start, in;
-  if (unit < split.total) {
-    if (!split.find(unit, &p->q, &p->request, &start)) return false;
-    p->splits = ceil_of(p->q.blocks, chunk);
-    in = (unit - start) / p->splits;
-    p->split = (unit - start) - in * p->splits;
-    p->slot = unit - p->split;
+// Split number `unit`; request -1 past the last one.
+template <typename LANES>
+__device__ __forceinline__ TilePart find_part(LANES& lanes, int unit, int chunk) {
+  Line<LANES, SplitsOf> split(lanes, SplitsOf{chunk, 1});
+  TilePart p;
+  p.request = -1;
+  const bool several = unit < split.total;
+  int start = 0, number = -1, x = unit;
+  bool found;
+  if (several) {
+    found = split.find(x, &p.q, &number, &start);
   } else {
-    Line<kTile, KEYS, SplitsOf<KEYS>> whole(a, SplitsOf<KEYS>{chunk, 0});
-    if (!whole.find(unit - split.total, &p->q, &p->request, &start)) return false;
-    in = unit - split.total - start;
-    p->splits = 1;
-    p->split = p->slot = 0;
+    x -= split.total;
+    Line<LANES, SplitsOf> whole(lanes, SplitsOf{chunk, 0});
+    found = whole.find(x, &p.q, &number, &start);
   }
-  p->place = p->q.tiles - 1 - in;
+  if (!found) return p;
+  p.splits = several ? ceil_of(p.q.blocks, chunk) : 1;
+  const int in = (x - start) / p.splits;
+  p.split = (x - start) - in * p.splits;
+  p.slot = several ? unit - p.split : 0;
+  p.place = p.q.tiles - 1 - in;
   // (sums that starts which do not ascend have wrapped must not lead outside the request or the workspace)
-  return p->place >= 0 && in >= 0 && (p->splits == 1 || (p->slot >= 0 && p->slot + p->splits <= 2 * a.units));
+  if (p.place >= 0 && in >= 0 && (!several || (p.slot >= 0 && p.slot + p.splits <= lanes.a.slots))) p.request = number;
+  return p;
 }
 
 // A tile's blocks: from *first on, as many as are returned, of KEYS keys.
@@ -979,9 +994,10 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_tile_kernel
   __shared__ __attribute__((aligned(16))) char k0l[KEYS * 2 * D], k1l[KEYS * 2 * D], v0l[KEYS * 2 * D], v1l[KEYS * 2 * D];
   const int head = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  TilePart s;
-  const int chunk = tile_chunk<KEYS>(a);
-  if (!find_part<KEYS>(a, blockIdx.x / a.Hkv, chunk, &s)) return;
+  Lanes<kTile, KEYS> lanes(a);
+  const int chunk = tile_chunk(lanes, kTileLeast / KEYS);
+  const TilePart s = find_part(lanes, blockIdx.x / a.Hkv, chunk);
+  if (s.request < 0) return;
   int tile_first, tile_last, low, block0;
   const int all = tile_blocks<KEYS>(a, s.q, s.place, &tile_first, &tile_last, &low, &block0);
   const int splits = max(1, ceil_of(ceil_of(all, 1 << a.grain), chunk));  // of this tile
@@ -1218,22 +1234,25 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_tile_kernel
   if (h == 0) a.state[result] = make_float2(top, sum);
 }
 
-// For attend_tile_kernel: a workgroup per 16 queries of a tile, at work where the unit is a tile's first split.
+// For attend_tile_kernel: a workgroup per split again, which takes its share of the tile's queries, 16 at a
+// time.
 template <int D>
 __global__ __launch_bounds__(kThreads) void merge_tile_kernel(AttendArgs a) {
   __shared__ float4 sums[kThreads / (D / 4)][4][D / 4];
   __shared__ float totals[kThreads / (D / 4)][4];
   constexpr int KEYS = tile_block<D>();
   const int head = blockIdx.x % a.Hkv;
-  const int chunk = tile_chunk<KEYS>(a);
-  TilePart s;
-  if (!find_part<KEYS>(a, blockIdx.x / a.Hkv, chunk, &s) || s.split || s.splits == 1) return;
+  Lanes<kTile, KEYS> lanes(a);
+  const int chunk = tile_chunk(lanes, kTileLeast / KEYS);
+  const TilePart s = find_part(lanes, blockIdx.x / a.Hkv, chunk);
+  if (s.request < 0 || s.splits == 1) return;
   int tile_first, tile_last, low, block0;
   const int all = tile_blocks<KEYS>(a, s.q, s.place, &tile_first, &tile_last, &low, &block0);
   const int splits = ceil_of(ceil_of(all, 1 << a.grain), chunk);
-  if (splits <= 1) return;
+  if (splits <= 1 || s.split >= splits) return;
   const int64_t slot = s.slot;
-  merge_tile<kTile, D>(a, s.q, s.place, head, kMergeQueries * blockIdx.y, splits, [&](int i) { return slot + i; }, sums, totals);
+  for (int i = s.split; i < kTile / kMergeQueries; i += splits)
+    merge_tile<kTile, D>(a, s.q, s.place, head, kMergeQueries * i, splits, [&](int j) { return slot + j; }, sums, totals);
 }
 
 // ------------------------------------------------------------ host side
@@ -1282,10 +1301,11 @@ int32_t check_heads(int32_t rows, int32_t Hq, int32_t Hkv, int32_t head_dim) {
   return IMQ_OK;
 }
 
-// A launch for the requests with `fewest` to `most` queries of a KV head (`width` 0: none): the parts it
-// shares their work out in, per KV head, and the tiles there may be.
+// A launch for the requests with `fewest` to `most` queries of a KV head, in tiles of `width` (0: none).  Per
+// KV head: the tiles there may be, the parts their work is shared out in, the workgroups, and the partial
+// results.
 struct AttendLaunch {
-  int64_t units, tiles;
+  int64_t tiles, units, workgroups, slots;
   int32_t fewest, most, width;
 };
 
@@ -1295,23 +1315,47 @@ struct AttendPlan {
 
 // Requests of up to kRowsMost queries go to attend_rows_kernel, longer ones to attend_tile_kernel.  The
 // host knows the sums only: where the average request stays within kRowsMost the first serves all.
-AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim) {
+// A workgroup with nothing to do costs its launch all the same (1000 of them 10 us): no more are launched than
+// the longest context can give work to.  The device makes do with what there is, whatever the contexts.
+AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim, int64_t max_context,
+                       int32_t window) {
   const int64_t queries = (int64_t)rows * (Hq / Hkv), with = std::min(rows, requests);
-  // at most one part-full tile for each request with rows
-  auto launch = [&](int workgroups, int width, int64_t fewest, int64_t most) {
-    return AttendLaunch{ceil_div(workgroups, Hkv), with + queries / width, (int32_t)fewest, (int32_t)most, width};
-  };
   AttendPlan p;
   memset(&p, 0, sizeof(p));
   const bool all_few = queries <= kRowsMost * with, some_few = requests > 1;
-  if (all_few || some_few) p.few = launch(head_dim == 128 ? kRowsWorkgroups<128> : kRowsWorkgroups<256>, kRowsTile, 0, all_few ? INT32_MAX : kRowsMost);
-  if (!all_few) p.many = launch(kTileWorkgroups, kTile, some_few ? kRowsMost + 1 : 0, INT32_MAX);
+  // (a window's keys before the rows' own, and the parts of blocks at both ends)
+  const int64_t keys = window ? std::min(max_context, (int64_t)window + rows) : max_context;
+  if (all_few || some_few) {
+    AttendLaunch& l = p.few;
+    l.width = kRowsTile;
+    l.most = all_few ? INT32_MAX : kRowsMost;
+    l.tiles = with + queries / kRowsTile;  // at most one part-full tile for each request with rows
+    const int64_t line = l.tiles * (keys / kRowsBlock + 2);
+    l.units = std::min<int64_t>(ceil_div(head_dim == 128 ? kRowsWorkgroups<128> : kRowsWorkgroups<256>, Hkv),
+                                ceil_div(line, kRowsLeast));
+    l.workgroups = l.units;
+    l.slots = l.units > 1 ? 2 * l.units : 0;  // a part's first tile and its last
+  }
+  if (!all_few) {
+    AttendLaunch& l = p.many;
+    l.width = kTile;
+    l.fewest = some_few ? kRowsMost + 1 : 0;
+    l.most = INT32_MAX;
+    l.tiles = with + queries / kTile;
+    const int keys_of = head_dim == 128 ? tile_block<128>() : tile_block<256>();
+    // the chunk is the work over the units and a tile has its blocks over the chunk, rounded up, of splits: no more
+    // than the units and the tiles together
+    const int64_t splits = ceil_div(keys / keys_of + 2, kTileLeast / keys_of);
+    l.workgroups = std::min(ceil_div(kTileWorkgroups, Hkv) + l.tiles, l.tiles * splits);
+    l.units = l.workgroups - l.tiles;
+    l.slots = std::min(l.workgroups, 2 * l.units);
+  }
   return p;
 }
 
 // The partial results' part of a launch's workspace, then their maxima and sums.
 size_t attend_space(const AttendLaunch& l, int32_t Hkv, int32_t head_dim) {
-  return (size_t)l.units * 2 * Hkv * l.width * (head_dim * 4 + 8);
+  return (size_t)l.slots * Hkv * l.width * (head_dim * 4 + 8);
 }
 
 // log2 of the blocks that the device counts as one: 0 unless the sums of the blocks of all tiles could pass 30 bits.
@@ -1327,9 +1371,10 @@ AttendArgs with_launch(AttendArgs a, const AttendLaunch& l, int head_dim, char* 
   a.fewest = l.fewest;
   a.most = l.most;
   a.units = (int32_t)l.units;
+  a.slots = (int32_t)l.slots;
   a.grain = attend_grain(l, (int64_t)a.columns << a.shift);
   a.partial = reinterpret_cast<float*>(space);
-  a.state = reinterpret_cast<float2*>(a.partial + (size_t)l.units * 2 * a.Hkv * l.width * head_dim);
+  a.state = reinterpret_cast<float2*>(a.partial + (size_t)l.slots * a.Hkv * l.width * head_dim);
   return a;
 }
 
@@ -1337,16 +1382,15 @@ template <int D>
 void launch_attend(const AttendPlan& p, char* space, const AttendArgs& args, hipStream_t stream) {
   if (p.few.width) {
     const AttendArgs a = with_launch(args, p.few, D, space);
-    const dim3 grid((uint32_t)(p.few.units * a.Hkv));
-    hipLaunchKernelGGL(attend_rows_kernel<D>, grid, dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(merge_rows_kernel<D>, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(attend_rows_kernel<D>, dim3((uint32_t)(p.few.workgroups * a.Hkv)), dim3(kThreads), 0, stream, a);
+    if (p.few.slots)
+      hipLaunchKernelGGL(merge_rows_kernel<D>, dim3((uint32_t)((p.few.units - 1) * a.Hkv)), dim3(kThreads), 0, stream, a);
   }
   if (p.many.width) {
     const AttendArgs a = with_launch(args, p.many, D, space + attend_space(p.few, args.Hkv, D));
-    // at most 2 units of the splits of tiles of several, and a workgroup for every other tile
-    const int64_t split = 2 * p.many.units;
-    hipLaunchKernelGGL(attend_tile_kernel<D>, dim3((uint32_t)((split + p.many.tiles) * a.Hkv)), dim3(kThreads), 0, stream, a);
-    hipLaunchKernelGGL(merge_tile_kernel<D>, dim3((uint32_t)(split * a.Hkv), kTile / kMergeQueries), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(attend_tile_kernel<D>, dim3((uint32_t)(p.many.workgroups * a.Hkv)), dim3(kThreads), 0, stream, a);
+    if (p.many.slots)
+      hipLaunchKernelGGL(merge_tile_kernel<D>, dim3((uint32_t)(p.many.slots * a.Hkv)), dim3(kThreads), 0, stream, a);
   }
 }
 
@@ -1431,8 +1475,8 @@ int32_t imq_paged_write(const uint16_t* q, int64_t ldq, const uint16_t* k, int64
 
 size_t imq_paged_attention_workspace(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim,
                                      int32_t max_context, int32_t window) {
-  if (check_heads(rows, Hq, Hkv, head_dim) != IMQ_OK || rows == 0 || requests < 1) return 0;
-  const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim);
+  if (check_heads(rows, Hq, Hkv, head_dim) != IMQ_OK || rows == 0 || requests < 1 || max_context < 1) return 0;
+  const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim, max_context, window);
   return attend_space(plan.few, Hkv, head_dim) + attend_space(plan.many, Hkv, head_dim);
 }
 
@@ -1455,12 +1499,13 @@ int32_t imq_paged_attention(const uint16_t* q, int64_t ldq, const uint16_t* k_pa
   for (const void* p : {(const void*)q, (const void*)k_pages, (const void*)v_pages, (const void*)out})
     if (!p || !aligned(p, 16)) return fail(IMQ_EINVAL, "rows and pages must be non-null and 16-byte aligned");
   if (!current_device(&code)) return code;
-  const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim);
-  if (!workspace || !aligned(workspace, 16) ||
-      workspace_bytes < attend_space(plan.few, Hkv, head_dim) + attend_space(plan.many, Hkv, head_dim))
+  const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim,
+                                      std::min<int64_t>(max_context, (int64_t)columns * page_size), window);
+  const size_t nbytes = attend_space(plan.few, Hkv, head_dim) + attend_space(plan.many, Hkv, head_dim);
+  if (nbytes && (!workspace || !aligned(workspace, 16) || workspace_bytes < nbytes))
     return fail(IMQ_EINVAL, "the workspace is too small or not 16-byte aligned");
   AttendArgs a{q, k_pages, v_pages, tables, starts, ends, out, ldq, ldo, nullptr, nullptr, rows, requests, columns, pages,
-               __builtin_ctz(page_size), Hq, Hkv, Hq / Hkv, window, 0, 0, 0, 0, scale * 1.44269504088896340736f};
+               __builtin_ctz(page_size), Hq, Hkv, Hq / Hkv, window, 0, 0, 0, 0, 0, scale * 1.44269504088896340736f};
   char* const space = static_cast<char*>(workspace);
   if (head_dim == 128)
     launch_attend<128>(plan, space, a, static_cast<hipStream_t>(stream));

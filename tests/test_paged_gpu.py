@@ -318,9 +318,10 @@ def test_long_and_wide_batches_against_64_bits(env, requests, heads, kv_heads, d
 def test_bounds_on_the_context_change_nothing(env):
     torch, n_ = env
     announce("paged attention, max_context")
-    b = _Batch(torch, [(1, 900), (1, 5), (3, 400)], 32, 8, 128, 16, seed=8)
-    for most in (900, 1 << 20, 901):
-        b.check(torch, n_, max_context=most)
+    for requests in ([(1, 900), (1, 5), (3, 400)], [(300, 900), (1, 2000)], [(200, 5000)]):
+        b = _Batch(torch, requests, 32, 8, 128, 16, seed=8)
+        for most in (5000, 1 << 20, 900, 64, 1):  # one that is too small only plans badly
+            b.check(torch, n_, max_context=most)
     with pytest.raises(n_.NativeError):
         b.run(n_, max_context=0)
 
