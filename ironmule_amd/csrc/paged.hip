@@ -556,7 +556,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t* odd) {
 // swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
 // over the softmax and P V, and no barrier before the wavefronts' results are joined.
-constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 4;
+constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 8;
 constexpr int kRowsMost = 32;  // queries of a request that attend_rows_kernel is there for
 template <int D>
 constexpr int kRowsWorkgroups = D == 128 ? 512 : 256;  // as many as are resident
@@ -802,25 +802,29 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_rows_kernel
   }
 }
 
-// The partial results of a tile added up in order.  A workgroup takes kMergeQueries queries of it, a group of D / 4 lanes
-// the partial results i, i + SG, ..: as many groups share a query as there are partial results for,
-// the others take other queries, four at a time.
-constexpr int kMergeQueries = 16;
+// The partial results of a tile added up: a group of D / 4 lanes takes four queries, and of up to
+// kMergeAlone partial results all, four at a time; of more, as many groups share the queries as there
+// are groups, each every so manieth, and their sums are added in LDS.  The queries are those of the passes
+// `pass`, `pass` + `step`, .. over the tile.  (A pass over maxima first, and LDS always, took 14 us where this takes 6.)
+constexpr int kMergeAlone = 8;
+
+template <int D>
+struct MergeSpace {
+  float4 sums[kThreads / (D / 4)][4][D / 4];
+  float tops[kThreads / (D / 4)][4], totals[kThreads / (D / 4)][4];
+};
 
 template <int WIDTH, int D, typename SLOT>
-__device__ __forceinline__ void merge_tile(const AttendArgs& a, const Request& s, int place, int head, int q0, int parts,
-                                           SLOT slot_of, float4 (*sums)[4][D / 4], float (*totals)[4]) {
+__device__ __forceinline__ void merge_part(const AttendArgs& a, const Request& s, int place, int head, int pass, int step,
+                                           int parts, SLOT slot_of, MergeSpace<D>& space) {
   constexpr int L = D / 4, NG = kThreads / L;
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
-  int share = 1;
-  while (share < NG && share < parts) share *= 2;
-  const int mine = group % share;
-  const int64_t step = (int64_t)a.Hkv * WIDTH;
-  for (int qb = 0; qb < kMergeQueries; qb += 4 * (NG / share)) {
-    const int first = WIDTH * place + q0 + qb;
-    if (first / a.group >= s.count) return;
-    const int q = q0 + qb + 4 * (group / share);  // and the three behind it
-    const bool some = q < q0 + kMergeQueries && (WIDTH * place + q) / a.group < s.count;
+  const int share = parts <= kMergeAlone ? 1 : NG, mine = group % share, many = 4 * (NG / share);
+  const int64_t slot_step = (int64_t)a.Hkv * WIDTH;
+  for (int qb = many * pass; qb < WIDTH; qb += many * step) {
+    if ((WIDTH * place + qb) / a.group >= s.count) return;
+    const int q = qb + 4 * (group / share);  // and the three behind it
+    const bool some = q < WIDTH && (WIDTH * place + q) / a.group < s.count;
     const int64_t at = (int64_t)head * WIDTH + q;
     float most[4], total[4];
     float4 v[4];
@@ -830,53 +834,78 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, const Request& s
       total[j] = 0.0f;
       v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    if (some) {
-      // (rows behind the request's last one have slots of their own that hold anything: not used)
-      for (int i = lane; i < parts; i += L)
+    // (rows behind the request's last one have places of their own that hold anything: not used)
+    for (int i0 = some ? mine : parts; i0 < parts; i0 += 4 * share) {
+      float2 st[4][4];
+      float4 u[4][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], a.state[at + j + slot_of(i) * step].x);
-#pragma unroll
-      for (int d = 1; d < L; d <<= 1)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) most[j] = fmaxf(most[j], __shfl_xor(most[j], d));
-#pragma unroll 2
-      for (int i = mine; i < parts; i += share) {
-        const int64_t from = at + slot_of(i) * step;
+      for (int k = 0; k < 4; ++k) {
+        const int64_t from = at + slot_of(min(i0 + k * share, parts - 1)) * slot_step;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float2 st = a.state[from + j];
-          const float w = exp2f(st.x - (most[j] == -INFINITY ? 0.0f : most[j]));
-          const float4 u = *reinterpret_cast<const float4*>(a.partial + (from + j) * D + 4 * lane);
-          total[j] = fmaf(st.y, w, total[j]);
-          v[j].x = fmaf(u.x, w, v[j].x);
-          v[j].y = fmaf(u.y, w, v[j].y);
-          v[j].z = fmaf(u.z, w, v[j].z);
-          v[j].w = fmaf(u.w, w, v[j].w);
+          st[k][j] = a.state[from + j];
+          u[k][j] = *reinterpret_cast<const float4*>(a.partial + (from + j) * D + 4 * lane);
         }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float higher = most[j];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) higher = fmaxf(higher, i0 + k * share < parts ? st[k][j].x : -INFINITY);
+        const float base = higher == -INFINITY ? 0.0f : higher, keep = exp2f(most[j] - base);
+        most[j] = higher;
+        total[j] *= keep;
+        v[j].x *= keep, v[j].y *= keep, v[j].z *= keep, v[j].w *= keep;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i0 + k * share < parts) {
+            const float w = exp2f(st[k][j].x - base);
+            total[j] = fmaf(st[k][j].y, w, total[j]);
+            v[j].x = fmaf(u[k][j].x, w, v[j].x);
+            v[j].y = fmaf(u[k][j].y, w, v[j].y);
+            v[j].z = fmaf(u[k][j].z, w, v[j].z);
+            v[j].w = fmaf(u[k][j].w, w, v[j].w);
+          }
+      }
+    }
+    auto write = [&](int j, const float4& r, float sum) {
+      const int query = WIDTH * place + q + j, row = query / a.group;
+      if (row >= s.count) return;
+      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+      const u32x2_t four = {pack_bf16(r.x * inv, r.y * inv), pack_bf16(r.z * inv, r.w * inv)};
+      *reinterpret_cast<u32x2_t*>(a.out + (s.first + row) * a.ldo + ((int64_t)head * a.group + query % a.group) * D + 4 * lane) = four;
+    };
+    if (share == 1) {
+      if (some)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) write(j, v[j], total[j]);
+      continue;
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      sums[group][j][lane] = v[j];
-      if (lane == 0) totals[group][j] = total[j];
+      space.sums[group][j][lane] = v[j];
+      if (lane == 0) space.tops[group][j] = most[j], space.totals[group][j] = total[j];
     }
     __syncthreads();
-    // the groups that shared a query write one of the four each
-    if (some)
-      for (int j = mine; j < 4; j += share) {
-        const int query = WIDTH * place + q + j, row = query / a.group;
-        if (row >= s.count) break;
-        float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        float t = 0.0f;
-        for (int k = 0; k < share; ++k) {
-          const float4 u = sums[group - mine + k][j][lane];
-          r.x += u.x, r.y += u.y, r.z += u.z, r.w += u.w;
-          t += totals[group - mine + k][j];
-        }
-        const float inv = t == 0.0f ? 0.0f : 1.0f / t;
-        const u32x2_t four = {pack_bf16(r.x * inv, r.y * inv), pack_bf16(r.z * inv, r.w * inv)};
-        *reinterpret_cast<u32x2_t*>(a.out + (s.first + row) * a.ldo + ((int64_t)head * a.group + query % a.group) * D + 4 * lane) = four;
+    if (some && group < 4) {  // one of the four queries each
+      const int j = group;
+      float higher = -INFINITY, sum = 0.0f;
+      float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int k = 0; k < NG; ++k) higher = fmaxf(higher, space.tops[k][j]);
+      const float base = higher == -INFINITY ? 0.0f : higher;
+#pragma unroll
+      for (int k = 0; k < NG; ++k) {
+        const float w = exp2f(space.tops[k][j] - base);
+        const float4 x = space.sums[k][j][lane];
+        sum = fmaf(space.totals[k][j], w, sum);
+        r.x = fmaf(x.x, w, r.x);
+        r.y = fmaf(x.y, w, r.y);
+        r.z = fmaf(x.z, w, r.z);
+        r.w = fmaf(x.w, w, r.w);
       }
+      write(j, r, sum);
+    }
     __syncthreads();
   }
 }
@@ -885,8 +914,7 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, const Request& s
 // the first inside its tile.
 template <int D>
 __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
-  __shared__ float4 sums[kThreads / (D / 4)][4][D / 4];
-  __shared__ float totals[kThreads / (D / 4)][4];
+  __shared__ MergeSpace<D> space;
   const int head = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv + 1;
   Lanes<kRowsTile, kRowsBlock> lanes(a);
   Line<Lanes<kRowsTile, kRowsBlock>, BlocksOf> line(lanes, BlocksOf());
@@ -899,8 +927,8 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
   if (tile == unit * part || tile < (unit - 1) * part) return;
   const int first = unit - 1, last = (tile + q.blocks - 1) / part;
   if (unit * part < start || place >= q.tiles || last >= a.units) return;  // (as in attend_rows_kernel)
-  merge_tile<kRowsTile, D>(a, q, place, head, 0, last - first + 1,
-                           [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 && tile > first * part)); }, sums, totals);
+  merge_part<kRowsTile, D>(a, q, place, head, 0, 1, last - first + 1,
+                           [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 && tile > first * part)); }, space);
 }
 
 // Many queries per request (chunks of prompts): tiles of 128 queries of one KV head, each of a workgroup's
@@ -1234,12 +1262,10 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_tile_kernel
   if (h == 0) a.state[result] = make_float2(top, sum);
 }
 
-// For attend_tile_kernel: a workgroup per split again, which takes its share of the tile's queries, 16 at a
-// time.
+// For attend_tile_kernel: a workgroup per split again, which takes its share of the tile's queries.
 template <int D>
 __global__ __launch_bounds__(kThreads) void merge_tile_kernel(AttendArgs a) {
-  __shared__ float4 sums[kThreads / (D / 4)][4][D / 4];
-  __shared__ float totals[kThreads / (D / 4)][4];
+  __shared__ MergeSpace<D> space;
   constexpr int KEYS = tile_block<D>();
   const int head = blockIdx.x % a.Hkv;
   Lanes<kTile, KEYS> lanes(a);
@@ -1251,8 +1277,7 @@ __global__ __launch_bounds__(kThreads) void merge_tile_kernel(AttendArgs a) {
   const int splits = ceil_of(ceil_of(all, 1 << a.grain), chunk);
   if (splits <= 1 || s.split >= splits) return;
   const int64_t slot = s.slot;
-  for (int i = s.split; i < kTile / kMergeQueries; i += splits)
-    merge_tile<kTile, D>(a, s.q, s.place, head, kMergeQueries * i, splits, [&](int j) { return slot + j; }, sums, totals);
+  merge_part<kTile, D>(a, s.q, s.place, head, s.split, splits, splits, [&](int i) { return slot + i; }, space);
 }
 
 // ------------------------------------------------------------ host side
