@@ -537,6 +537,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // v_cvt_pk
 }
 
 typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
+typedef __attribute__((address_space(3))) u32x4_t* lds_u32x4;
+typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
+typedef __attribute__((address_space(3))) char* lds_char;
+__device__ __forceinline__ uint32_t lds_at(char* p) { return (uint32_t)(uintptr_t)(lds_char)p; }
 // (page numbers of a whole wavefront, which no kernel that reads them writes: loaded by the scalar unit)
 typedef const __attribute__((address_space(4))) int32_t* scalar_ints;
 
@@ -557,7 +561,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t* odd) {
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
 // over the softmax and P V, and no barrier before the wavefronts' results are joined.
 constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 8;
-constexpr int kRowsMost = 32;  // queries of a request that attend_rows_kernel is there for
+constexpr int kRowsMost = 32;  // queries of a request that rows_workgroup is there for
 template <int D>
 constexpr int kRowsWorkgroups = D == 128 ? 512 : 256;  // as many as are resident
 constexpr int kTileWorkgroups = 512;
@@ -567,13 +571,24 @@ __device__ __forceinline__ int part_length(const AttendArgs& a, int total, int l
   return max(least, (total + a.units - 1) / a.units);
 }
 
+// The LDS of a workgroup of either kind: four arrays of 16 KB (of their own: a read of one does not wait for
+// the loads into another), for attend_rows a block's values of each wavefront and then its result.
+constexpr int kArray = 16384;
+
+// Wavefront w's part of it.
 template <int D>
-__device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& s, int request, int place, int from, int to,
-                                            int slot, char* lds, float (*tops)[16], float (*sums)[16]) {
+__device__ __forceinline__ lds_char part_of(int w, uint32_t at0, uint32_t at1, uint32_t at2, uint32_t at3) {
+  if (D == 128) return (lds_char)(uintptr_t)((w & 2 ? at1 : at0) + (w & 1) * (32 * 2 * D));
+  return (lds_char)(uintptr_t)(w & 2 ? (w & 1 ? at3 : at2) : w & 1 ? at1 : at0);
+}
+
+template <int D>
+__device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const Request& s, int request, int place, int from,
+                                            int to, int slot, char* l0, char* l1, char* l2, char* l3, float (*tops)[16],
+                                            float (*sums)[16]) {
   constexpr int T = D / 32, P = D / 8, C = D / 16;  // k-steps of a score, 16-byte pieces of a row, 16-dim tiles
   constexpr int V = 32 * P / 64;                    // 16-byte pieces of a block's values per lane
-  constexpr int kBytes = 32 * 2 * D;
-  const int head = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int query = 16 * place + n, row = query / a.group;
   const bool live = row < s.count;
@@ -584,6 +599,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
   const int low = a.window ? max(0, tile_first - a.window + 1) : 0;
   const int64_t q_head = (int64_t)head * a.group + query % a.group;
 
+  const uint32_t at0 = lds_at(l0), at1 = lds_at(l1), at2 = D == 128 ? 0u : lds_at(l2), at3 = D == 128 ? 0u : lds_at(l3);
   // the wavefront's blocks: its quarter of those between from and to that the tile sees
   from = max(from, low / kRowsBlock);
   to = tile_last < low ? from : min(to, tile_last / kRowsBlock + 1);
@@ -607,7 +623,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
     const scalar_ints table = (scalar_ints)(a.tables + (int64_t)request * a.columns);
     const int mask = (1 << a.shift) - 1;
     const uint32_t k_lane = 2 * (n * D + 8 * g), v_lane = 2 * ((lane / P) * D + 8 * (lane % P));
-    char* const vl = lds + wave * kBytes;
+    const lds_char vl = part_of<D>(wave, at0, at1, at2, at3);
 
     // the pages of a block's two 16-key groups (a page holds a multiple of 16 tokens).  (Plain numbers, no
     // array: as one they went to LDS, for whose layout the compiler has every workgroup read the launch's
@@ -669,7 +685,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         const int r = (64 / P) * i + lane / P, piece = lane % P;
-        *reinterpret_cast<u32x4_t*>(vl + r * 2 * D + 32 * ((piece >> 1) ^ (r & 7)) + 16 * (piece & 1)) = vr[i];
+        *(lds_u32x4)(vl + r * 2 * D + 32 * ((piece >> 1) ^ (r & 7)) + 16 * (piece & 1)) = vr[i];
       }
       load_v(next0, next1, ahead);
       const int after0 = page_of(min(at + 2, stop - 1), 0), after1 = page_of(min(at + 2, stop - 1), 1);
@@ -708,7 +724,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
         // lane i of each 16 reads 8 bytes of row i / 4; the transposed read gives it the four rows' value
         // of dimension i
         const int r = 4 * g + (n >> 2);
-        char* const v0 = vl + r * 2 * D + 32 * (c ^ (r & 7)) + 8 * (n & 3);
+        const lds_char v0 = vl + r * 2 * D + 32 * (c ^ (r & 7)) + 8 * (n & 3);
         const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)v0);
         const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v0 + 16 * 2 * D));
         const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -747,10 +763,9 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
   __syncthreads();  // (and every wavefront is through with its values in LDS)
   const float most = fmaxf(fmaxf(tops[0][n], tops[1][n]), fmaxf(tops[2][n], tops[3][n]));
   const float scale = exp2f(top - (most == -INFINITY ? 0.0f : most));
-  float4* const joined = reinterpret_cast<float4*>(lds);  // (wavefront, tile of 16 dims, lane): 4 kBytes
 #pragma unroll
   for (int c = 0; c < C; ++c)
-    joined[(wave * C + c) * 64 + lane] = make_float4(o[c][0] * scale, o[c][1] * scale, o[c][2] * scale, o[c][3] * scale);
+    ((lds_f32x4)part_of<D>(wave, at0, at1, at2, at3))[c * 64 + lane] = o[c] * scale;  // (tile of 16 dims, lane)
   __syncthreads();
   float total = 0.0f;
 #pragma unroll
@@ -760,28 +775,25 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, const Request& 
 #pragma unroll
   for (int i = 0; i < C / 4; ++i) {
     const int c = wave + 4 * i;
-    float4 v = joined[c * 64 + lane];
+    f32x4_t v = ((lds_f32x4)part_of<D>(0, at0, at1, at2, at3))[c * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-      const float4 u = joined[(w * C + c) * 64 + lane];
-      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-    }
+    for (int w = 1; w < 4; ++w) v += ((lds_f32x4)part_of<D>(w, at0, at1, at2, at3))[c * 64 + lane];
     if (!live) continue;
     if (slot < 0) {
       const u32x2_t four = {pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv)};
       *reinterpret_cast<u32x2_t*>(a.out + (s.first + row) * a.ldo + q_head * D + 16 * c + 4 * g) = four;
     } else {
-      *reinterpret_cast<float4*>(a.partial + result * D + 16 * c + 4 * g) = v;
+      *reinterpret_cast<f32x4_t*>(a.partial + result * D + 16 * c + 4 * g) = v;
     }
   }
   if (slot >= 0 && live && wave == 0 && g == 0) a.state[result] = make_float2(most, total);
 }
 
+// Workgroup `index` of a launch over tiles of few queries.
 template <int D>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * 32 * 2 * D];
-  __shared__ float tops[4][16], sums[4][16];
-  const int unit = blockIdx.x / a.Hkv;
+__device__ __forceinline__ void rows_workgroup(const AttendArgs& a, int index, char* l0, char* l1, char* l2, char* l3,
+                                               float (*tops)[16], float (*sums)[16]) {
+  const int unit = index / a.Hkv, head = index % a.Hkv;
   Lanes<kRowsTile, kRowsBlock> lanes(a);
   Line<Lanes<kRowsTile, kRowsBlock>, BlocksOf> line(lanes, BlocksOf());
   const int part = part_length(a, line.total, kRowsLeast);
@@ -797,7 +809,8 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_rows_kernel
     // a tile not whole here: the workgroup's first partial result, or its last
     const int slot = length == q.blocks ? -1 : 2 * unit + (x != x0);
     if (x != x0) __syncthreads();
-    attend_rows<D>(a, q, request, place, q.block0 + (in << a.grain), q.block0 + ((in + length) << a.grain), slot, lds, tops, sums);
+    attend_rows<D>(a, head, q, request, place, q.block0 + (in << a.grain), q.block0 + ((in + length) << a.grain), slot, l0, l1, l2, l3,
+                   tops, sums);
     x += length;
   }
 }
@@ -910,12 +923,11 @@ __device__ __forceinline__ void merge_part(const AttendArgs& a, const Request& s
   }
 }
 
-// For attend_rows_kernel: a workgroup per boundary between two parts of the line, at work where it is
+// After rows_workgroup: a workgroup per boundary between two parts of the line, at work where it is
 // the first inside its tile.
 template <int D>
-__global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
-  __shared__ MergeSpace<D> space;
-  const int head = blockIdx.x % a.Hkv, unit = blockIdx.x / a.Hkv + 1;
+__device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, MergeSpace<D>& space) {
+  const int head = index % a.Hkv, unit = index / a.Hkv + 1;
   Lanes<kRowsTile, kRowsBlock> lanes(a);
   Line<Lanes<kRowsTile, kRowsBlock>, BlocksOf> line(lanes, BlocksOf());
   const int part = part_length(a, line.total, kRowsLeast);
@@ -926,7 +938,7 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
   const int place = (unit * part - start) / q.blocks, tile = start + place * q.blocks;
   if (tile == unit * part || tile < (unit - 1) * part) return;
   const int first = unit - 1, last = (tile + q.blocks - 1) / part;
-  if (unit * part < start || place >= q.tiles || last >= a.units) return;  // (as in attend_rows_kernel)
+  if (unit * part < start || place >= q.tiles || last >= a.units) return;  // (as in rows_workgroup)
   merge_part<kRowsTile, D>(a, q, place, head, 0, 1, last - first + 1,
                            [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 && tile > first * part)); }, space);
 }
@@ -939,7 +951,7 @@ __global__ __launch_bounds__(kThreads) void merge_rows_kernel(AttendArgs a) {
 // a score passes it by 2^8: until then the probabilities are up to 256, which costs no accuracy, and the
 // sums need not be scaled again.  K lies in LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both
 // swizzled so that the rows that a read takes at a time lie in different banks (the 32-byte pieces of
-// attend_rows_kernel and K's by row & 7 had every read conflict once: half of the LDS cycles).
+// attend_rows and K's by row & 7 had every read conflict once: half of the LDS cycles).
 //
 // A tile is cut into splits of at most `chunk` blocks, the chunk such that there are about kTileWorkgroups
 // of them.  Tiles of requests that have several splits come first, and a request's last tiles, the longest,
@@ -1013,18 +1025,18 @@ __device__ __forceinline__ int tile_blocks(const AttendArgs& a, const Request& q
   return *tile_last < *low ? 0 : *tile_last / KEYS + 1 - *first;
 }
 
+// Workgroup `index` of a launch over tiles of many queries.
 template <int D>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_tile_kernel(AttendArgs a) {
+__device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, char* k0l, char* k1l, char* v0l, char* v1l) {
   constexpr int KEYS = tile_block<D>(), B = KEYS / 32, T = D / 16, C = D / 32, P = D / 8;
   constexpr int MINE = KEYS / 4, L = MINE * P / 64;  // keys of a block that a wavefront loads, 1 KB at a time
   constexpr int GROUPS = KEYS / 16;
-  // (arrays of their own: a read of one does not wait for the loads into another)
-  __shared__ __attribute__((aligned(16))) char k0l[KEYS * 2 * D], k1l[KEYS * 2 * D], v0l[KEYS * 2 * D], v1l[KEYS * 2 * D];
-  const int head = blockIdx.x % a.Hkv, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  static_assert(KEYS * 2 * D == kArray, "a block's keys, or its values, fill an array");
+  const int head = index % a.Hkv, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Lanes<kTile, KEYS> lanes(a);
   const int chunk = tile_chunk(lanes, kTileLeast / KEYS);
-  const TilePart s = find_part(lanes, blockIdx.x / a.Hkv, chunk);
+  const TilePart s = find_part(lanes, index / a.Hkv, chunk);
   if (s.request < 0) return;
   int tile_first, tile_last, low, block0;
   const int all = tile_blocks<KEYS>(a, s.q, s.place, &tile_first, &tile_last, &low, &block0);
@@ -1262,15 +1274,14 @@ __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_tile_kernel
   if (h == 0) a.state[result] = make_float2(top, sum);
 }
 
-// For attend_tile_kernel: a workgroup per split again, which takes its share of the tile's queries.
+// After tile_workgroup: a workgroup per split again, which takes its share of the tile's queries.
 template <int D>
-__global__ __launch_bounds__(kThreads) void merge_tile_kernel(AttendArgs a) {
-  __shared__ MergeSpace<D> space;
+__device__ __forceinline__ void merge_tile(const AttendArgs& a, int index, MergeSpace<D>& space) {
   constexpr int KEYS = tile_block<D>();
-  const int head = blockIdx.x % a.Hkv;
+  const int head = index % a.Hkv;
   Lanes<kTile, KEYS> lanes(a);
   const int chunk = tile_chunk(lanes, kTileLeast / KEYS);
-  const TilePart s = find_part(lanes, blockIdx.x / a.Hkv, chunk);
+  const TilePart s = find_part(lanes, index / a.Hkv, chunk);
   if (s.request < 0 || s.splits == 1) return;
   int tile_first, tile_last, low, block0;
   const int all = tile_blocks<KEYS>(a, s.q, s.place, &tile_first, &tile_last, &low, &block0);
@@ -1278,6 +1289,49 @@ __global__ __launch_bounds__(kThreads) void merge_tile_kernel(AttendArgs a) {
   if (splits <= 1 || s.split >= splits) return;
   const int64_t slot = s.slot;
   merge_part<kTile, D>(a, s.q, s.place, head, s.split, splits, splits, [&](int i) { return slot + i; }, space);
+}
+
+// A launch for requests of few queries, of many, or of both: `few_groups` and `many_groups` workgroups.
+// With both, eight of one kind and eight of the other in turn (an XCD gets workgroups of both), so that those that
+// wait for memory and those that multiply share the CUs: the mixed batch of 24 in 138 us one after the other.
+enum { kFew = 1, kMany = 2 };
+
+__device__ __forceinline__ int own_index(int block, int few_groups, int many_groups, bool* few) {
+  const int both = min(few_groups, many_groups) & ~7;  // of either kind in turn
+  if (block < 2 * both) {
+    *few = !(block & 8);
+    return (block >> 4) * 8 + (block & 7);
+  }
+  block -= both;
+  *few = block < few_groups;
+  return *few ? block : block - few_groups + both;
+}
+
+template <int D, int KINDS>
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_kernel(AttendArgs few, AttendArgs many, int few_groups,
+                                                                            int many_groups) {
+  __shared__ __attribute__((aligned(16))) char lds0[kArray], lds1[kArray];
+  __shared__ float tops[4][16], sums[4][16];
+  if (KINDS == kFew && D == 128) {
+    rows_workgroup<D>(few, blockIdx.x, lds0, lds1, nullptr, nullptr, tops, sums);
+  } else {
+    __shared__ __attribute__((aligned(16))) char lds2[kArray], lds3[kArray];
+    bool is_few = KINDS == kFew;
+    const int index = KINDS == (kFew | kMany) ? own_index(blockIdx.x, few_groups, many_groups, &is_few) : blockIdx.x;
+    if ((KINDS & kFew) && is_few)
+      rows_workgroup<D>(few, index, lds0, lds1, lds2, lds3, tops, sums);
+    else if (KINDS & kMany)
+      tile_workgroup<D>(many, index, lds0, lds1, lds2, lds3);
+  }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void merge_kernel(AttendArgs few, AttendArgs many, int few_groups) {
+  __shared__ MergeSpace<D> space;
+  if ((int)blockIdx.x < few_groups)
+    merge_rows<D>(few, blockIdx.x, space);
+  else
+    merge_tile<D>(many, blockIdx.x - few_groups, space);
 }
 
 // ------------------------------------------------------------ host side
@@ -1338,7 +1392,7 @@ struct AttendPlan {
   AttendLaunch few, many;
 };
 
-// Requests of up to kRowsMost queries go to attend_rows_kernel, longer ones to attend_tile_kernel.  The
+// Requests of up to kRowsMost queries go to rows_workgroup, longer ones to tile_workgroup.  The
 // host knows the sums only: where the average request stays within kRowsMost the first serves all.
 // A workgroup with nothing to do costs its launch all the same (1000 of them 10 us): no more are launched than
 // the longest context can give work to.  The device makes do with what there is, whatever the contexts.
@@ -1405,18 +1459,16 @@ AttendArgs with_launch(AttendArgs a, const AttendLaunch& l, int head_dim, char* 
 
 template <int D>
 void launch_attend(const AttendPlan& p, char* space, const AttendArgs& args, hipStream_t stream) {
-  if (p.few.width) {
-    const AttendArgs a = with_launch(args, p.few, D, space);
-    hipLaunchKernelGGL(attend_rows_kernel<D>, dim3((uint32_t)(p.few.workgroups * a.Hkv)), dim3(kThreads), 0, stream, a);
-    if (p.few.slots)
-      hipLaunchKernelGGL(merge_rows_kernel<D>, dim3((uint32_t)((p.few.units - 1) * a.Hkv)), dim3(kThreads), 0, stream, a);
-  }
-  if (p.many.width) {
-    const AttendArgs a = with_launch(args, p.many, D, space + attend_space(p.few, args.Hkv, D));
-    hipLaunchKernelGGL(attend_tile_kernel<D>, dim3((uint32_t)(p.many.workgroups * a.Hkv)), dim3(kThreads), 0, stream, a);
-    if (p.many.slots)
-      hipLaunchKernelGGL(merge_tile_kernel<D>, dim3((uint32_t)(p.many.slots * a.Hkv)), dim3(kThreads), 0, stream, a);
-  }
+  const AttendArgs few = with_launch(args, p.few, D, space);
+  const AttendArgs many = with_launch(args, p.many, D, space + attend_space(p.few, args.Hkv, D));
+  const int few_groups = (int)p.few.workgroups * args.Hkv, many_groups = (int)p.many.workgroups * args.Hkv;
+  const auto kernel = !p.many.width  ? attend_kernel<D, kFew>
+                      : !p.few.width ? attend_kernel<D, kMany>
+                                     : attend_kernel<D, (kFew | kMany)>;
+  hipLaunchKernelGGL(kernel, dim3(few_groups + many_groups), dim3(kThreads), 0, stream, few, many, few_groups, many_groups);
+  const int few_merges = p.few.slots ? (int)(p.few.units - 1) * args.Hkv : 0, many_merges = (int)p.many.slots * args.Hkv;
+  if (few_merges + many_merges)
+    hipLaunchKernelGGL(merge_kernel<D>, dim3(few_merges + many_merges), dim3(kThreads), 0, stream, few, many, few_merges);
 }
 
 bool row_stride(int64_t ld, int64_t width) { return ld >= width && ld % 8 == 0; }
