@@ -563,8 +563,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t* odd) {
 constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 8;
 constexpr int kRowsMost = 32;  // queries of a request that rows_workgroup is there for
 template <int D>
-constexpr int kRowsWorkgroups = D == 128 ? 512 : 256;  // as many as are resident
-constexpr int kTileWorkgroups = 512;
+constexpr int kWorkgroups = D == 128 ? 512 : 256;  // as many as are resident
 
 // The length of a part of the line.
 __device__ __forceinline__ int part_length(const AttendArgs& a, int total, int least) {
@@ -923,8 +922,8 @@ __device__ __forceinline__ void merge_part(const AttendArgs& a, const Request& s
   }
 }
 
-// After rows_workgroup: a workgroup per boundary between two parts of the line, at work where it is
-// the first inside its tile.
+// After rows_workgroup: a workgroup per boundary between two parts of the line; those inside a tile
+// share its queries.
 template <int D>
 __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, MergeSpace<D>& space) {
   const int head = index % a.Hkv, unit = index / a.Hkv + 1;
@@ -936,10 +935,10 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
   int request, start;
   if (!line.find(unit * part, &q, &request, &start)) return;
   const int place = (unit * part - start) / q.blocks, tile = start + place * q.blocks;
-  if (tile == unit * part || tile < (unit - 1) * part) return;
-  const int first = unit - 1, last = (tile + q.blocks - 1) / part;
+  if (tile == unit * part) return;
+  const int first = tile / part, last = (tile + q.blocks - 1) / part;  // the parts that hold some of it
   if (unit * part < start || place >= q.tiles || last >= a.units) return;  // (as in rows_workgroup)
-  merge_part<kRowsTile, D>(a, q, place, head, 0, 1, last - first + 1,
+  merge_part<kRowsTile, D>(a, q, place, head, unit - first - 1, last - first, last - first + 1,
                            [&](int i) { return (int64_t)(2 * (first + i) + (i == 0 && tile > first * part)); }, space);
 }
 
@@ -953,10 +952,14 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
 // swizzled so that the rows that a read takes at a time lie in different banks (the 32-byte pieces of
 // attend_rows and K's by row & 7 had every read conflict once: half of the LDS cycles).
 //
-// A tile is cut into splits of at most `chunk` blocks, the chunk such that there are about kTileWorkgroups
-// of them.  Tiles of requests that have several splits come first, and a request's last tiles, the longest,
+// A tile is cut into splits of at most `chunk` blocks, the chunk such that there are about as many
+// as workgroups are resident.  Tiles of requests that have several splits come first, and a request's last tiles, the longest,
 // before its first ones.
-constexpr int kTile = 128, kTileLeast = 512;  // (keys)
+//
+// A block takes a workgroup alone on its CU 0.7 us, two of them 1.45 together; a launch's start, the first
+// block with its instructions still to be fetched, and its end 8, the second launch 5.  So no tile is split where
+// the longest context has kTileAlone keys or fewer.
+constexpr int kTile = 128, kTileLeast = 256, kTileAlone = 1024;  // (keys)
 constexpr float kSlack = 8.0f;
 
 template <int D>
@@ -1402,6 +1405,7 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
   AttendPlan p;
   memset(&p, 0, sizeof(p));
   const bool all_few = queries <= kRowsMost * with, some_few = requests > 1;
+  const int resident = head_dim == 128 ? kWorkgroups<128> : kWorkgroups<256>;
   // (a window's keys before the rows' own, and the parts of blocks at both ends)
   const int64_t keys = window ? std::min(max_context, (int64_t)window + rows) : max_context;
   if (all_few || some_few) {
@@ -1410,7 +1414,7 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
     l.most = all_few ? INT32_MAX : kRowsMost;
     l.tiles = with + queries / kRowsTile;  // at most one part-full tile for each request with rows
     const int64_t line = l.tiles * (keys / kRowsBlock + 2);
-    l.units = std::min<int64_t>(ceil_div(head_dim == 128 ? kRowsWorkgroups<128> : kRowsWorkgroups<256>, Hkv),
+    l.units = std::min<int64_t>(ceil_div(resident, Hkv),
                                 ceil_div(line, kRowsLeast));
     l.workgroups = l.units;
     l.slots = l.units > 1 ? 2 * l.units : 0;  // a part's first tile and its last
@@ -1424,8 +1428,8 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
     const int keys_of = head_dim == 128 ? tile_block<128>() : tile_block<256>();
     // the chunk is the work over the units and a tile has its blocks over the chunk, rounded up, of splits: no more
     // than the units and the tiles together
-    const int64_t splits = ceil_div(keys / keys_of + 2, kTileLeast / keys_of);
-    l.workgroups = std::min(ceil_div(kTileWorkgroups, Hkv) + l.tiles, l.tiles * splits);
+    const int64_t splits = keys <= kTileAlone ? 1 : ceil_div(keys / keys_of + 2, kTileLeast / keys_of);
+    l.workgroups = std::min(ceil_div(resident, Hkv) + l.tiles, l.tiles * splits);
     l.units = l.workgroups - l.tiles;
     l.slots = std::min(l.workgroups, 2 * l.units);
   }
