@@ -34,13 +34,17 @@ __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo 
 // the k-th page asked for (requests in order, a request's columns in order) is the k-th lowest page
 // with no references.
 //   1. A thread per request: its columns to write, its first page if others hold it too.
-//   2. A thread per column to write, 1024 at a time: whether it needs a page; a scan over the threads
-//      gives its rank, left in the table as -2 - rank.
-//   3. The free pages, kWindow at a time in LDS, by a scan over the references (which ends where enough
-//      are found); then a thread per column again: rank -> page, or -1 again for a refused request.
+//   2. A thread per COLUMNS columns to write: which need a page; a scan over the threads gives their
+//      ranks, left in the table as -2 - rank.
+//   3. The free pages, WINDOW at a time in LDS, by a scan over the references (which ends where enough
+//      are found); then a thread per COLUMNS columns again: rank -> page, or -1 again for a refused request.
 // Requests are taken or refused between the two by the sums of what was asked for.
-constexpr int kReserveThreads = 1024;
-constexpr int kWindow = 8192;  // free pages listed at a time
+//
+// Bound by its chain of loads and barriers, and in a large cache by the references, which one CU reads
+// at about 150 GB/s (512 KB for 131072 pages).  One column and four references a thread at a time are best for
+// a step's few columns (eight beams 5.6 us, 9.6 with eight and 16), those for many prompts' (a round of 764 requests 50, 104 with
+// the others).
+constexpr int kReserveThreads = 1024, kReserveWaves = kReserveThreads / 64;
 constexpr int kMaxRequests = IMQ_PAGED_MAX_REQUESTS;
 
 struct ReserveArgs {
@@ -64,38 +68,66 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 
-// Inclusive scan over the workgroup's WAVES wavefronts; *total gets the sum.  `part`: WAVES ints of
-// LDS, free again when the call returns.
+// Inclusive sums over a workgroup of WAVES wavefronts, one barrier each: the two halves of `part` take turns,
+// and nobody writes one of them again before the barrier of the other.
 template <int WAVES>
-__device__ __forceinline__ int group_scan(int v, int* part, int* total) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  v = wave_scan(v);
-  if (lane == 63) part[wave] = v;
-  __syncthreads();
-  int before = 0, all = 0;
+struct GroupScan {
+  int (*part)[WAVES];
+  int turn = 0;
+  __device__ __forceinline__ int operator()(int v, int* total) {
+    const int wave = threadIdx.x >> 6;
+    int* const mine = part[turn];
+    turn ^= 1;
+    v = wave_scan(v);
+    if ((threadIdx.x & 63) == 63) mine[wave] = v;
+    __syncthreads();
+    int before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) {
-    const int p = part[w];
-    before += w < wave ? p : 0;
-    all += p;
+    for (int w = 0; w < WAVES; ++w) {
+      const int p = mine[w];
+      before += w < wave ? p : 0;
+      all += p;
+    }
+    *total = all;
+    return v + before;
   }
-  __syncthreads();
-  *total = all;
-  return v + before;
-}
+};
 
+template <int COLUMNS, int REFS, int WINDOW>
 __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(ReserveArgs a) {
-  __shared__ int part[kReserveThreads / 64];
-  __shared__ int list[kWindow];
-  __shared__ int last_item[kMaxRequests];   // columns to write, up to and with this request
+  __shared__ int part[2][kReserveWaves];
+  __shared__ int list[WINDOW];
+  __shared__ int last_item[kMaxRequests];  // columns to write, up to and with this request
   __shared__ int first_col[kMaxRequests];
-  __shared__ int old_page[kMaxRequests];    // the shared page this request leaves, -1 none
+  __shared__ int old_page[kMaxRequests];   // the shared page this request leaves, -1 none
   __shared__ int new_page[kMaxRequests];
   __shared__ int before_wants[kMaxRequests], after_wants[kMaxRequests];
-  __shared__ int bad_table[kMaxRequests], refused[kMaxRequests];
+  __shared__ int flags[kMaxRequests];      // 1: a shared page past its tokens; 2: refused
   const int tid = threadIdx.x;
   const bool mine = tid < a.requests;
-  const int waves = kReserveThreads / 64;
+  GroupScan<kReserveWaves> scan{part};
+  auto four_refs = [&](int p) {
+    int4 v = make_int4(1, 1, 1, 1);
+    if (p + 3 < a.pages) {
+      v = *reinterpret_cast<const int4*>(a.refs + p);
+    } else {
+      if (p < a.pages) v.x = a.refs[p];
+      if (p + 1 < a.pages) v.y = a.refs[p + 1];
+      if (p + 2 < a.pages) v.z = a.refs[p + 2];
+    }
+    return v;
+  };
+  auto free_of = [&](int p) {  // which of the REFS pages from p on are free
+    int4 v[REFS / 4];
+#pragma unroll
+    for (int i = 0; i < REFS / 4; ++i) v[i] = four_refs(p + 4 * i);
+    uint32_t free = 0;
+#pragma unroll
+    for (int i = 0; i < REFS / 4; ++i)
+      free |= (uint32_t)((v[i].x == 0) | (v[i].y == 0) << 1 | (v[i].z == 0) << 2 | (v[i].w == 0) << 3) << (4 * i);
+    return free;
+  };
+  const uint32_t first_free = free_of(REFS * tid);  // (on its way over the first step's loads)
 
   // 1. a thread per request
   int len = 0, count = 0, items = 0, old = -1;
@@ -115,16 +147,16 @@ __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(ReserveArgs a)
     old_page[tid] = old;
     new_page[tid] = -1;
     before_wants[tid] = after_wants[tid] = 0;
-    bad_table[tid] = 0;
+    flags[tid] = 0;
   }
-  int all_items, all_rows;
-  const int upto = group_scan<waves>(items, part, &all_items);
+  int all_items;
+  const int upto = scan(items, &all_items);
   if (mine) last_item[tid] = upto;
   // rows asked for: more than there are count as one more, which keeps the sums in 32 bits
-  const int rows_upto = group_scan<waves>(count < a.rows ? count : a.rows + (count > a.rows), part, &all_rows);
-  __syncthreads();
+  int all_rows;
+  const int rows_upto = scan(count < a.rows ? count : a.rows + (count > a.rows), &all_rows);
 
-  auto request_of = [&](int item) {  // the first request whose last column lies past `item`
+  auto request_of = [&](int item) {  // the first request whose last column lies past the item
     int lo = 0, hi = a.requests - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -132,116 +164,119 @@ __global__ __launch_bounds__(kReserveThreads) void reserve_kernel(ReserveArgs a)
     }
     return lo;
   };
+  // The columns to write `item` .. item + COLUMNS - 1, the first of request lo: work(j, request, number in it, whether
+  // its last, entry).
+  auto for_items = [&](int item, int lo, auto work) {
+#pragma unroll
+    for (int j = 0; j < COLUMNS; ++j) {
+      if (item + j >= all_items) break;
+      while (last_item[lo] <= item + j) ++lo;
+      const int place = item + j - (lo ? last_item[lo - 1] : 0);
+      work(j, lo, place, item + j + 1 == last_item[lo], a.tables + (int64_t)lo * a.columns + first_col[lo] + place);
+    }
+  };
 
-  // 2. a thread per column to write
+  // 2. the columns that need a page
   int wanted = 0;
-  for (int base = 0; base < all_items; base += kReserveThreads) {
-    const int item = base + tid;
-    int r = 0, place = 0, need = 0;
-    int32_t* entry = nullptr;
-    if (item < all_items) {
-      r = request_of(item);
-      place = item - (r ? last_item[r - 1] : 0);
-      entry = a.tables + (int64_t)r * a.columns + first_col[r] + place;
-      const int cur = *entry;
-      const bool held = cur >= 0 && cur < a.pages;
-      need = !held || (place == 0 && old_page[r] >= 0);
-      if (held && place && a.refs[cur] > 1) bad_table[r] = 1;
-    }
-    int sum;
-    const int rank = wanted + group_scan<waves>(need, part, &sum);  // inclusive
-    if (entry) {
-      if (need) *entry = -2 - (rank - 1);
-      if (place == 0) before_wants[r] = rank - need;
-      if (item + 1 == last_item[r]) after_wants[r] = rank;
-    }
+  for (int base = 0; base < all_items; base += COLUMNS * kReserveThreads) {
+    const int item = base + COLUMNS * tid;
+    const int lo = request_of(item);
+    int32_t current[COLUMNS], need[COLUMNS] = {}, sum;
+    for_items(item, lo, [&](int j, int, int, bool, int32_t* entry) { current[j] = *entry; });
+    int n = 0;
+    for_items(item, lo, [&](int j, int r, int place, bool, int32_t*) {
+      const bool held = current[j] >= 0 && current[j] < a.pages;
+      need[j] = !held || (place == 0 && old_page[r] >= 0);
+      n += need[j];
+      if (held && place && a.refs[current[j]] > 1) flags[r] = 1;
+    });
+    int rank = wanted + scan(n, &sum) - n;
+    for_items(item, lo, [&](int j, int r, int place, bool last, int32_t* entry) {
+      if (need[j]) *entry = -2 - rank;
+      if (place == 0) before_wants[r] = rank;
+      rank += need[j];
+      if (last) after_wants[r] = rank;
+    });
     wanted += sum;
   }
 
-  // 3. the free pages
-  int cursor = 0;  // pages below it are listed already, or in use
-  auto fill = [&](int most) {  // lists up to min(most, kWindow) free pages; returns how many
+  // 3. the free pages: lists up to min(most, WINDOW) from `cursor` on; returns how many
+  int cursor = 0;
+  auto fill = [&](int most) {
     int have = 0;
-    const int want = most < kWindow ? most : kWindow;
-    int at = cursor & ~3;
-    while (at < a.pages && have < want) {
-      const int p = at + 4 * tid;
-      int free[4], sum;
-      int4 v = make_int4(1, 1, 1, 1);
-      if (p + 3 < a.pages) {
-        v = *reinterpret_cast<const int4*>(a.refs + p);
-      } else {
-        if (p < a.pages) v.x = a.refs[p];
-        if (p + 1 < a.pages) v.y = a.refs[p + 1];
-        if (p + 2 < a.pages) v.z = a.refs[p + 2];
-      }
-      free[0] = v.x == 0 && p >= cursor;
-      free[1] = v.y == 0 && p + 1 >= cursor;
-      free[2] = v.z == 0 && p + 2 >= cursor;
-      free[3] = v.w == 0 && p + 3 >= cursor;
-      const int n = free[0] + free[1] + free[2] + free[3];
-      int to = have + group_scan<waves>(n, part, &sum) - n;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (free[e]) {
-          if (to < want) list[to] = p + e;
-          ++to;
-        }
+    const int want = most < WINDOW ? most : WINDOW;
+    for (int at = cursor & ~3; at < a.pages && have < want; at += REFS * kReserveThreads) {
+      const int p = at + REFS * tid;
+      uint32_t free = at == 0 ? first_free : free_of(p);
+      if (p < cursor) free &= cursor - p < 32 ? ~0u << (cursor - p) : 0u;
+      const int n = __popc(free);
+      int sum, to = have + scan(n, &sum) - n;
+      for (; free; free &= free - 1, ++to)
+        if (to < want) list[to] = p + __builtin_ctz(free);
       have += sum;
-      at += 4 * kReserveThreads;
     }
     __syncthreads();
     if (have > want) have = want;
     if (have) cursor = list[have - 1] + 1;
     return have;
   };
-  int found = 0;
-  while (found < wanted) {
-    const int n = fill(wanted - found);
-    found += n;
-    if (n == 0) break;
-    if (found < wanted) __syncthreads();  // the list is filled again
+  const bool one_window = wanted <= WINDOW;
+  int found;
+  if (one_window) {
+    found = wanted ? fill(wanted) : 0;
+  } else {
+    int n = 0, all;
+    for (int p = REFS * tid; p < a.pages; p += REFS * kReserveThreads) n += __popc(free_of(p));
+    scan(n, &all);
+    found = min(wanted, all);
   }
-  const bool one_window = wanted <= kWindow;
+  __syncthreads();
 
   // taken or refused
   int state = 0;
   if (mine) {
     const bool short_of = after_wants[tid] > before_wants[tid] && after_wants[tid] > found;
-    state = malformed || bad_table[tid] ? 2 : short_of ? 1 : count && rows_upto > a.rows ? 3 : 0;
-    refused[tid] = state != 0;
+    state = malformed || flags[tid] ? 2 : short_of ? 1 : count && rows_upto > a.rows ? 3 : 0;
+    if (state) flags[tid] = 2;
     a.status[tid] = state;
     a.ends[tid] = state ? len : len + count;
   }
   int all_taken;
-  const int taken = group_scan<waves>(state ? 0 : count, part, &all_taken);
+  const int taken = scan(state ? 0 : count, &all_taken);
   if (mine) a.starts[tid + 1] = taken;
   if (tid == 0) a.starts[0] = 0;
-  __syncthreads();
 
   // rank -> page
-  cursor = 0;
-  int window = 0;
-  do {
-    const int n = one_window ? found : fill(wanted - window);
-    for (int item = tid; item < all_items; item += kReserveThreads) {
-      const int r = request_of(item), place = item - (r ? last_item[r - 1] : 0);
-      int32_t* const entry = a.tables + (int64_t)r * a.columns + first_col[r] + place;
-      const int rank = -2 - *entry;
-      if (rank < 0) continue;
-      if (refused[r]) {
-        *entry = place == 0 ? old_page[r] : -1;
-      } else if (rank >= window && rank < window + n) {
-        const int page = list[rank - window];
-        *entry = page;
-        a.refs[page] = 1;
-        if (place == 0) new_page[r] = page;
-      }
+  int window = 0, listed = one_window ? found : 0;  // the list holds ranks window .. window + listed - 1
+  for (int base = 0; base < all_items; base += COLUMNS * kReserveThreads) {
+    const int item = base + COLUMNS * tid;
+    const int lo = request_of(item);
+    int32_t code[COLUMNS] = {};
+    for_items(item, lo, [&](int j, int, int, bool, int32_t* entry) { code[j] = *entry; });
+    for (;;) {
+      bool later = false;
+      for_items(item, lo, [&](int j, int r, int place, bool, int32_t* entry) {
+        const int rank = -2 - code[j];
+        if (rank < 0) return;
+        if (flags[r]) {
+          *entry = place == 0 ? old_page[r] : -1;
+        } else if (rank >= window + listed) {
+          later = true;
+          return;
+        } else {
+          const int page = list[rank - window];
+          *entry = page;
+          a.refs[page] = 1;
+          if (place == 0) new_page[r] = page;
+        }
+        code[j] = 0;
+      });
+      if (one_window || !__syncthreads_or(later)) break;
+      window += listed;
+      listed = fill(found - window);
+      if (listed == 0) break;
     }
-    window += n;
-    if (n == 0) break;
-    __syncthreads();
-  } while (window < found);
+  }
   __syncthreads();
   if (mine) {
     int from = -1, to = -1;
@@ -265,7 +300,7 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const int32_t* __restric
                                                         int columns, int pages, int shift, int rows, int row_groups,
                                                         int planes, int64_t page_bytes) {
   __shared__ int table[2 * kMaxRequests + 1];
-  __shared__ int part[kThreads / 64];
+  __shared__ int part[2][kThreads / 64];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x < row_groups) {
     for (int i = tid; i <= requests; i += kThreads) table[i] = starts[i];
@@ -287,13 +322,14 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const int32_t* __restric
     return;
   }
   // the requests that copy, in order
+  GroupScan<kThreads / 64> scan{part};
   int copied = 0;
   for (int base = 0; base < requests; base += kThreads) {
     const int r = base + tid;
     const int from = r < requests ? copies[2 * r] : -1, to = r < requests ? copies[2 * r + 1] : -1;
     const int some = from >= 0;
     int sum;
-    const int at = copied + group_scan<kThreads / 64>(some, part, &sum) - 1;
+    const int at = copied + scan(some, &sum) - 1;
     if (some) table[2 * at] = from, table[2 * at + 1] = to;
     copied += sum;
   }
@@ -311,34 +347,53 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const int32_t* __restric
 
 // ------------------------------------------------------------ reordering of requests
 //
-// A workgroup takes some columns of every request: it reads them all into LDS, then writes each
-// request's from its parent's and counts the pages that come and go.  The counts are integers, so
-// the order of the additions does not matter.  The lengths follow in a launch of their own: every
-// workgroup reads the parents' old ones.
+// A workgroup takes some columns of every request: it reads them all into LDS, with each request's
+// parent and how many columns that one holds, then writes each request's from its parent's and counts the
+// pages that come and go.  The counts are integers, so the order of the additions does not matter.  One
+// workgroup does small tables and the lengths with them; for larger ones the lengths follow in a launch
+// of their own, since every workgroup reads the parents' old ones.  (With up to 8192 entries and 256 threads a
+// workgroup 73 requests of 258 columns took 14 us.)
 constexpr int kReorderEntries = 8192;  // table entries of a workgroup, 32 KB of LDS
+constexpr int kReorderThreads = 1024;
 
-__global__ __launch_bounds__(kThreads) void reorder_kernel(int32_t* __restrict__ tables,
-                                                           const int32_t* __restrict__ lengths,
-                                                           int32_t* __restrict__ refs,
-                                                           const int32_t* __restrict__ parents, int requests, int columns,
-                                                           int pages, int shift, int width) {
+__device__ __forceinline__ bool changes(int r, int parent, int requests) {
+  return parent != r && parent >= -1 && parent < requests;
+}
+
+__global__ __launch_bounds__(kReorderThreads) void reorder_kernel(int32_t* __restrict__ tables, int32_t* __restrict__ lengths,
+                                                                  int32_t* __restrict__ refs,
+                                                                  const int32_t* __restrict__ parents, int requests,
+                                                                  int columns, int pages, int shift, int log2_width,
+                                                                  int whole) {
   __shared__ int old[kReorderEntries];
-  const int c0 = blockIdx.x * width, wide = min(width, columns - c0), entries = requests * wide;
-  for (int e = threadIdx.x; e < entries; e += kThreads)
-    old[e] = tables[(int64_t)(e / wide) * columns + c0 + e % wide];
+  __shared__ int parent[kMaxRequests], held[kMaxRequests];  // the columns that the request will hold
+  const int width = 1 << log2_width, c0 = blockIdx.x << log2_width, entries = requests << log2_width, tid = threadIdx.x;
+  int length = 0;
+  if (tid < requests) {
+    const int p = parents[tid];
+    if (p >= 0 && p < requests) length = lengths[p];
+    parent[tid] = p;
+    held[tid] = length > 0 ? (int)(((int64_t)length + (1 << shift) - 1) >> shift) : 0;
+  }
+#pragma unroll 4
+  for (int e = tid; e < entries; e += kReorderThreads) {
+    const int r = e >> log2_width, c = c0 + (e & (width - 1));
+    old[e] = c < columns ? tables[(int64_t)r * columns + c] : -1;
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < entries; e += kThreads) {
-    const int r = e / wide, c = e % wide, p = parents[r];
-    if (p == r || p < -1 || p >= requests) continue;
+#pragma unroll 4
+  for (int e = tid; e < entries; e += kReorderThreads) {
+    const int r = e >> log2_width, in = e & (width - 1), p = parent[r];
+    if (c0 + in >= columns || !changes(r, p, requests)) continue;
     const int before = old[e];
-    int after = -1;
-    if (p >= 0 && (int64_t)lengths[p] > ((int64_t)(c0 + c) << shift)) after = old[p * wide + c];
+    int after = p >= 0 && c0 + in < held[r] ? old[(p << log2_width) + in] : -1;
     if (after < 0 || after >= pages) after = -1;
     if (before == after) continue;
     if (before >= 0 && before < pages) atomicSub(refs + before, 1);
     if (after >= 0) atomicAdd(refs + after, 1);
-    tables[(int64_t)r * columns + c0 + c] = after;
+    tables[(int64_t)r * columns + c0 + in] = after;
   }
+  if (whole && tid < requests && changes(tid, parent[tid], requests)) lengths[tid] = length;
 }
 
 __global__ __launch_bounds__(kMaxRequests) void reorder_lengths_kernel(int32_t* __restrict__ lengths,
@@ -348,7 +403,7 @@ __global__ __launch_bounds__(kMaxRequests) void reorder_lengths_kernel(int32_t* 
   bool change = false;
   if (r < requests) {
     const int p = parents[r];
-    change = p != r && p >= -1 && p < requests;
+    change = changes(r, p, requests);
     if (change && p >= 0) length = lengths[p];
   }
   __syncthreads();
@@ -1500,7 +1555,10 @@ int32_t imq_paged_reserve(const imq_paged_cache* cache, const int32_t* counts, c
   const int shift = __builtin_ctz(cache->page_size);
   ReserveArgs a{cache->tables, cache->lengths, cache->refs, counts, chunk->starts, chunk->ends, chunk->status,
                 chunk->copies, cache->requests, cache->columns, cache->pages, shift, chunk->rows};
-  hipLaunchKernelGGL(reserve_kernel, dim3(1), dim3(kReserveThreads), 0, st, a);
+  // at most this many columns: those that the rows fill, and two part-full ones for each request
+  const int64_t most = chunk->rows / cache->page_size + 2 * (int64_t)cache->requests;
+  const auto kernel = most <= 2 * kReserveThreads ? reserve_kernel<1, 4, 4096> : reserve_kernel<8, 16, 24576>;
+  hipLaunchKernelGGL(kernel, dim3(1), dim3(kReserveThreads), 0, st, a);
   code = launched("reserve");
   if (code != IMQ_OK) return code;
   const int row_groups = ceil_div(chunk->rows, kThreads);
@@ -1519,11 +1577,17 @@ int32_t imq_paged_reorder(const imq_paged_cache* cache, const int32_t* parents, 
   if (!parents) return fail(IMQ_EINVAL, "null pointer");
   if (!current_device(&code)) return code;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int width = std::min(cache->columns, std::min(256, kReorderEntries / cache->requests));
-  hipLaunchKernelGGL(reorder_kernel, dim3(ceil_div(cache->columns, width)), dim3(kThreads), 0, st, cache->tables,
-                     cache->lengths, cache->refs, parents, cache->requests, cache->columns, cache->pages,
-                     __builtin_ctz(cache->page_size), width);
-  hipLaunchKernelGGL(reorder_lengths_kernel, dim3(1), dim3(kMaxRequests), 0, st, cache->lengths, parents, cache->requests);
+  // columns of a workgroup: all where they fit, else 16 (or what fits), a 64-byte piece of a row
+  int log2_width = 0;
+  while ((1 << log2_width) < cache->columns) ++log2_width;
+  const bool whole = ((int64_t)cache->requests << log2_width) <= kReorderEntries;
+  if (!whole)
+    for (log2_width = 4; (cache->requests << log2_width) > kReorderEntries;) --log2_width;
+  hipLaunchKernelGGL(reorder_kernel, dim3(ceil_div(cache->columns, 1 << log2_width)), dim3(kReorderThreads), 0, st,
+                     cache->tables, cache->lengths, cache->refs, parents, cache->requests, cache->columns, cache->pages,
+                     __builtin_ctz(cache->page_size), log2_width, whole ? 1 : 0);
+  if (!whole)
+    hipLaunchKernelGGL(reorder_lengths_kernel, dim3(1), dim3(kMaxRequests), 0, st, cache->lengths, parents, cache->requests);
   return launched("reorder");
 }
 

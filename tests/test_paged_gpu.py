@@ -57,6 +57,9 @@ class _Device:
 
     def reserve(self, counts):
         torch, want_pool = self.torch, None
+        if self.chunk["positions"].numel() != self.rows:
+            for name in ("positions", "slots"):
+                self.chunk[name] = self.torch.full((self.rows,), -7, dtype=self.torch.int32, device="cuda")
         want = self.model.reserve(counts, self.rows)
         if self.pool is not None:
             want_pool = self.pool.clone()
@@ -120,18 +123,32 @@ def test_rounds_of_a_cache_agree_with_the_model(env, requests, columns, pages, p
 
 
 def test_more_pages_than_one_list_holds(env):
-    """9000 and 12000 pages in one call, more than are listed at a time; then a call for more than are left, with
-    a request refused in the middle of a list."""
+    """Some 60000 pages in one call, more than twice what is listed at a time; then calls for more than are left,
+    with requests refused in the middle of a list and behind it."""
     torch, n_ = env
     announce("paged reserve, long lists")
-    device = _Device(torch, n_, PagedModel(4, 13000, 40000, 16), 1 << 20)
-    device.reserve([9000 * 16, 1, 12000 * 16 - 3, 0])
+    device = _Device(torch, n_, PagedModel(5, 30000, 100003, 16), 1 << 20)
+    device.reserve([19000 * 16, 1, 22000 * 16 - 3, 0, 19000 * 16])
     device.commit()
-    device.reorder([0, 1, 2, 1])
-    device.reserve([13000 * 16 - 9000 * 16, 12999 * 16, 5, 12000 * 16])
+    device.reorder([0, 1, 2, 1, 4])
+    device.reserve([11000 * 16, 29999 * 16 - 5, 5, 12000 * 16, 1])
     device.commit()
-    device.reorder([-1, 0, 2, -1])
-    device.reserve([10000 * 16] * 2 + [1, 12000 * 16])
+    device.reorder([-1, 0, 2, -1, 4])
+    device.reorder([0, 1, -1, -1, -1])
+    device.rows = 0
+    want = device.reserve([30000 * 16] * 2 + [25000 * 16, 30000 * 16, 16])
+    assert 0 not in want["status"][2:]
+
+
+def test_lists_end_where_pages_do(env):
+    """Requests that fit the free pages exactly, by one page less and by one more, lists of several lengths."""
+    torch, n_ = env
+    announce("paged reserve, exact fits")
+    for pages in (3, 1000, 24576, 24577, 50000):
+        for over in (-1, 0, 1):
+            device = _Device(torch, n_, PagedModel(3, 60000, pages, 16), 1 << 20)
+            want = device.reserve([(pages // 3) * 16, 0, (pages - pages // 3 + over) * 16])
+            assert want["status"].tolist() == [0, 0, int(over > 0)]
 
 
 def test_a_shared_page_past_the_tokens_is_refused(env):
