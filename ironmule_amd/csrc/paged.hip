@@ -412,60 +412,106 @@ __global__ __launch_bounds__(kMaxRequests) void reorder_lengths_kernel(int32_t* 
 
 // ------------------------------------------------------------ norm, rotary, rows into pages
 //
-// A workgroup per row, a wavefront per head at a time; lane l holds dimensions l, l + 64, .. of the
-// head, so that the pairs (d, d + head_dim / 2) that turn together lie in one lane.
+// A workgroup per row, D / 16 lanes per head; lane l holds dimensions 8 l .. 8 l + 7 of the head and those
+// D / 2 further on, so that the pairs that turn together lie in one lane and every load and store is 16
+// bytes.  The first heads' loads are in flight while the row's angles are computed (in double: positions
+// are large, and the angle is the product).  Two roundings to bf16, as imq_qk_norm_rope: the norm's result
+// (what the model's norm gives) and the turned value.
+// Bound by memory: 4099 rows of 48 heads of 128 (134 MB read and written) in 22.5 us, 6.0 TB/s; single
+// 2-byte values a lane took 34.  The slot is looked at after the loads: before them, 32.  256 to 512
+// threads are alike there, 320 and more best for a few rows (five rows 3.8 us, 4.2 with 256); a number of
+// threads by the row's heads 26.
+constexpr int kWriteThreads = 384;
+
+typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // v_cvt_pk_bf16_f32
+  bf16x2v r;
+  r.x = (__bf16)lo;
+  r.y = (__bf16)hi;
+  return __builtin_bit_cast(uint32_t, r);
+}
+
+__device__ __forceinline__ float octets(const uint4 w, int i) {  // value i of eight bf16 values
+  const uint32_t word = i < 2 ? w.x : i < 4 ? w.y : i < 6 ? w.z : w.w;
+  return __uint_as_float(i & 1 ? word & 0xffff0000u : word << 16);
+}
+
 template <int D>
-__global__ __launch_bounds__(kThreads) void write_kernel(const uint16_t* __restrict__ q, int64_t ldq,
-                                                         const uint16_t* __restrict__ k, int64_t ldk,
-                                                         const uint16_t* __restrict__ v, int64_t ldv,
-                                                         const uint16_t* __restrict__ q_norm,
-                                                         const uint16_t* __restrict__ k_norm,
-                                                         const int32_t* __restrict__ positions,
-                                                         const int32_t* __restrict__ slots, uint16_t* __restrict__ q_out,
-                                                         int64_t ldo, uint16_t* __restrict__ k_pages,
-                                                         uint16_t* __restrict__ v_pages, int Hq, int Hkv, int shift,
-                                                         int64_t tokens, double log2_theta, float eps) {
-  constexpr int H = D / 2, N = D / 64;
-  __shared__ float turn[2][H];
-  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int slot = slots[row];
-  if (slot < 0 || slot >= tokens) return;
-  if (threadIdx.x < H) {
+__global__ __launch_bounds__(kWriteThreads) void write_kernel(const uint16_t* __restrict__ q, int64_t ldq,
+                                                              const uint16_t* __restrict__ k, int64_t ldk,
+                                                              const uint16_t* __restrict__ v, int64_t ldv,
+                                                              const uint16_t* __restrict__ q_norm,
+                                                              const uint16_t* __restrict__ k_norm,
+                                                              const int32_t* __restrict__ positions,
+                                                              const int32_t* __restrict__ slots,
+                                                              uint16_t* __restrict__ q_out, int64_t ldo,
+                                                              uint16_t* __restrict__ k_pages,
+                                                              uint16_t* __restrict__ v_pages, int Hq, int Hkv,
+                                                              int shift, int64_t tokens, double log2_theta, float eps) {
+  constexpr int H = D / 2, L = D / 16;  // L lanes a head
+  __shared__ __align__(16) float turn[2][H];
+  const int row = blockIdx.x, slot = slots[row], in = threadIdx.x % L;
+  const int heads = Hq + 2 * Hkv, stride = kWriteThreads / L;
+  int hh = threadIdx.x / L;
+  uint4 lo, hi;
+  const auto load = [&] {
+    const uint16_t* const src = hh < Hq         ? q + row * ldq + hh * D
+                                : hh < Hq + Hkv ? k + row * ldk + (hh - Hq) * D
+                                                : v + row * ldv + (hh - Hq - Hkv) * D;
+    lo = *reinterpret_cast<const uint4*>(src + 8 * in);
+    hi = *reinterpret_cast<const uint4*>(src + H + 8 * in);
+  };
+  if (hh < heads) load();
+  for (int d = threadIdx.x; d < H; d += kWriteThreads) {
     double sn, cs;
-    sincos((double)positions[row] * exp2(-(double)threadIdx.x * (log2_theta / H)), &sn, &cs);
-    turn[0][threadIdx.x] = (float)sn;
-    turn[1][threadIdx.x] = (float)cs;
+    sincos((double)positions[row] * exp2(-(double)d * (log2_theta / H)), &sn, &cs);
+    turn[0][d] = (float)sn;
+    turn[1][d] = (float)cs;
   }
   __syncthreads();
-  const int page = slot >> shift, offset = slot & ((1 << shift) - 1);
-  for (int hh = wave; hh < Hq + 2 * Hkv; hh += kThreads / 64) {
+  if (slot < 0 || slot >= tokens) return;
+  const int64_t page = slot >> shift, offset = slot & ((1 << shift) - 1);
+  while (hh < heads) {
     const bool is_q = hh < Hq, is_v = hh >= Hq + Hkv;
     const int head = is_q ? hh : is_v ? hh - Hq - Hkv : hh - Hq;
-    const uint16_t* const src = is_q ? q + row * ldq + head * D : is_v ? v + row * ldv + head * D : k + row * ldk + head * D;
     uint16_t* const dst = is_q ? q_out + row * ldo + head * D
-                               : (is_v ? v_pages : k_pages) + ((((int64_t)page * Hkv + head) << shift) + offset) * D;
-    if (is_v) {
+                               : (is_v ? v_pages : k_pages) + (((page * Hkv + head) << shift) + offset) * D;
+    uint4 lo_out = lo, hi_out = hi;
+    if (!is_v) {
+      float x[16], ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) dst[lane + 64 * i] = src[lane + 64 * i];
-      continue;
+      for (int i = 0; i < 8; ++i) {
+        x[i] = octets(lo, i);
+        x[8 + i] = octets(hi, i);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+      for (int step = 1; step < L; step *= 2) ss += __shfl_xor(ss, step);
+      const float inv = 1.0f / sqrtf(ss / (float)D + eps);
+      const uint16_t* const weight = is_q ? q_norm : k_norm;
+      const uint4 w_lo = *reinterpret_cast<const uint4*>(weight + 8 * in);
+      const uint4 w_hi = *reinterpret_cast<const uint4*>(weight + H + 8 * in);
+      uint32_t made[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = pack_bf16(x[2 * i] * inv * octets(w_lo, 2 * i), x[2 * i + 1] * inv * octets(w_lo, 2 * i + 1));
+        const uint32_t b = pack_bf16(x[8 + 2 * i] * inv * octets(w_hi, 2 * i), x[9 + 2 * i] * inv * octets(w_hi, 2 * i + 1));
+        const float2 s = *reinterpret_cast<const float2*>(&turn[0][8 * in + 2 * i]);
+        const float2 c = *reinterpret_cast<const float2*>(&turn[1][8 * in + 2 * i]);
+        const float a0 = __uint_as_float(a << 16), a1 = __uint_as_float(a & 0xffff0000u);
+        const float b0 = __uint_as_float(b << 16), b1 = __uint_as_float(b & 0xffff0000u);
+        made[0][i] = pack_bf16(a0 * c.x - b0 * s.x, a1 * c.y - b1 * s.y);
+        made[1][i] = pack_bf16(a0 * s.x + b0 * c.x, a1 * s.y + b1 * c.y);
+      }
+      lo_out = make_uint4(made[0][0], made[0][1], made[0][2], made[0][3]);
+      hi_out = make_uint4(made[1][0], made[1][1], made[1][2], made[1][3]);
     }
-    const uint16_t* const weight = is_q ? q_norm : k_norm;
-    float x[N], ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x[i] = bf16_bits_to_f32(src[lane + 64 * i]);
-      ss = fmaf(x[i], x[i], ss);
-    }
-    const float inv = 1.0f / sqrtf(wave_sum(ss) / (float)D + eps);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      x[i] = bf16_bits_to_f32(f32_to_bf16_bits(x[i] * inv * bf16_bits_to_f32(weight[lane + 64 * i])));
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      const float lo = x[i], hi = x[i + N / 2], s = turn[0][lane + 64 * i], c = turn[1][lane + 64 * i];
-      dst[lane + 64 * i] = f32_to_bf16_bits(lo * c - hi * s);
-      dst[lane + 64 * i + H] = f32_to_bf16_bits(lo * s + hi * c);
-    }
+    *reinterpret_cast<uint4*>(dst + 8 * in) = lo_out;
+    *reinterpret_cast<uint4*>(dst + H + 8 * in) = hi_out;
+    hh += stride;
+    if (hh < heads) load();
   }
 }
 
@@ -582,15 +628,6 @@ struct BlocksOf {
 __device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef __bf16 bf16x2v __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {  // v_cvt_pk_bf16_f32
-  bf16x2v r;
-  r.x = (__bf16)lo;
-  r.y = (__bf16)hi;
-  return __builtin_bit_cast(uint32_t, r);
-}
-
 typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4_t* lds_u32x4;
 typedef __attribute__((address_space(3))) f32x4_t* lds_f32x4;
@@ -1613,7 +1650,7 @@ int32_t imq_paged_write(const uint16_t* q, int64_t ldq, const uint16_t* k, int64
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int shift = __builtin_ctz(page_size);
   const auto kernel = head_dim == 128 ? write_kernel<128> : write_kernel<256>;
-  hipLaunchKernelGGL(kernel, dim3(rows), dim3(kThreads), 0, st, q, ldq, k, ldk, v, ldv, q_norm, k_norm, positions, slots,
+  hipLaunchKernelGGL(kernel, dim3(rows), dim3(kWriteThreads), 0, st, q, ldq, k, ldk, v, ldv, q_norm, k_norm, positions, slots,
                      q_out, ldo, k_pages, v_pages, Hq, Hkv, shift, (int64_t)pages << shift, log2(theta), eps);
   return launched("paged write");
 }
