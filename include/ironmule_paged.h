@@ -82,7 +82,7 @@ IMQ_API int32_t imq_paged_reorder(const imq_paged_cache* cache, const int32_t* p
 
 /* Per row and head: q and k heads get the per-head RMSNorm (q_norm / k_norm weights of head_dim
  * values, rounded to bf16) and the non-interleaved rotary embedding at positions[row] with base
- * theta; q goes to q_out (rows ldo apart), k and the untouched v to the pages at slots[row].
+ * theta; q goes to q_out (rows ldo apart; q itself, or memory of its own), k and the untouched v to the pages at slots[row].
  * q, k, v: rows of heads * head_dim values ldq, ldk, ldv apart.  head_dim 128 or 256.  A row whose
  * slot is outside the pages (padding, a refused request) is left out: nothing is written for it.
  * Slots of one call are distinct.  The paged form of imq_qk_norm_rope. */

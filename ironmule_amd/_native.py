@@ -406,15 +406,29 @@ def _workspace(nbytes: int, device, stream) -> torch.Tensor:
     return ws
 
 
-def _grouped_launch(probs, count: int, m: int, dtype: torch.dtype, device, stream) -> None:
-    """imq_qmv_grouped, through imq_qmv_grouped_ws with this stream's workspace when the
+def qmv_workspace_bytes(shapes) -> int:
+    """Bytes of a zero-filled workspace that serves qmv_grouped for up to three weights of these (N, K)
+    at a time, at any number of rows."""
+    probs = (Problem * 3)()
+    need = 0
+    for i in range(len(shapes)):
+        for count in range(1, min(3, len(shapes) - i) + 1):
+            for p, (n, k) in zip(probs, shapes[i:i + count]):
+                p.ldx = p.K = k
+                p.ldy = p.N = n
+            need = max(need, *(int(lib().imq_qmv_grouped_workspace(probs, count, m)) for m in range(3, MAX_ROWS + 1)))
+    return need
+
+
+def _grouped_launch(probs, count: int, m: int, dtype: torch.dtype, device, stream, workspace=None) -> None:
+    """imq_qmv_grouped, through imq_qmv_grouped_ws with this stream's workspace (or the given one) when the
     library wants one (M >= 3 and few rows: the groups are split over more workgroups)."""
     nbytes = int(lib().imq_qmv_grouped_workspace(probs, count, m)) if m >= 3 else 0
     if nbytes == 0:
         _check(lib().imq_qmv_grouped(probs, count, m, GROUP_SIZE, BITS, _DTYPE_CODE[dtype],
                                      _stream(stream)))
         return
-    ws = _workspace(nbytes, device, stream)
+    ws = _workspace(nbytes, device, stream) if workspace is None else workspace
     _check(lib().imq_qmv_grouped_ws(probs, count, m, GROUP_SIZE, BITS, _DTYPE_CODE[dtype],
                                     _ptr(ws), ws.numel() * 4, _stream(stream)))
 
@@ -443,9 +457,12 @@ def qmv_multi(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
 
 def qmv_grouped(weights: list[tuple[torch.Tensor, torch.Tensor, torch.Tensor]],
                 xs: list[torch.Tensor], outs: list[torch.Tensor] | None = None,
-                out_dtype: torch.dtype = torch.bfloat16, stream=None) -> list[torch.Tensor]:
+                out_dtype: torch.dtype = torch.bfloat16, stream=None,
+                workspace: torch.Tensor | None = None) -> list[torch.Tensor]:
     """One launch for up to 8 weights, each with its own (M, K_i) activation rows (the
-    same tensor may serve several weights, e.g. q/k/v); returns the (M, N_i) outputs."""
+    same tensor may serve several weights, e.g. q/k/v); returns the (M, N_i) outputs.  `workspace`: fp32,
+    zero before its first use, in place of the stream's own (qmv_workspace_bytes; calls that share one
+    must not overlap)."""
     count = len(weights)
     if not 1 <= count <= MAX_PROBLEMS or len(xs) != count:
         raise ValueError(f"1 to {MAX_PROBLEMS} weights with one activation each")
@@ -476,7 +493,7 @@ def qmv_grouped(weights: list[tuple[torch.Tensor, torch.Tensor, torch.Tensor]],
         result.append(y)
     if not 1 <= m <= MAX_ROWS:
         raise ValueError(f"the qmv kernels take 1 to {MAX_ROWS} rows, got {m}")
-    _grouped_launch(probs, count, m, out_dtype, weights[0][0].device, stream)
+    _grouped_launch(probs, count, m, out_dtype, weights[0][0].device, stream, workspace)
     return result
 
 
@@ -790,8 +807,8 @@ def paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: torch
                 positions: torch.Tensor, slots: torch.Tensor, q_out: torch.Tensor, k_pages: torch.Tensor,
                 v_pages: torch.Tensor, theta: float, eps: float) -> torch.Tensor:
     """Per-head RMSNorm and rotary embedding of q and k (imq_paged_write), on the current stream: q (rows, heads,
-    head_dim) to q_out, k and v (rows, kv_heads, head_dim) to the pages at `slots`; rows whose slot is
-    outside the pages are left out.  Rows may lie apart (a slice of a wider projection)."""
+    head_dim) to q_out (may be q itself), k and v (rows, kv_heads, head_dim) to the pages at `slots`; rows
+    whose slot is outside the pages are left out.  Rows may lie apart (a slice of a wider projection)."""
     pages, kv_heads, page_size, dim = _pages_shape(k_pages, v_pages)
     ldq, ldk, ldv, ldo = (_head_rows(*x) for x in (("q", q), ("k", k), ("v", v), ("q_out", q_out)))
     rows, heads, _ = q.shape

@@ -438,14 +438,14 @@ __device__ __forceinline__ float octets(const uint4 w, int i) {  // value i of e
 }
 
 template <int D>
-__global__ __launch_bounds__(kWriteThreads) void write_kernel(const uint16_t* __restrict__ q, int64_t ldq,
+__global__ __launch_bounds__(kWriteThreads) void write_kernel(const uint16_t* q, int64_t ldq,
                                                               const uint16_t* __restrict__ k, int64_t ldk,
                                                               const uint16_t* __restrict__ v, int64_t ldv,
                                                               const uint16_t* __restrict__ q_norm,
                                                               const uint16_t* __restrict__ k_norm,
                                                               const int32_t* __restrict__ positions,
                                                               const int32_t* __restrict__ slots,
-                                                              uint16_t* __restrict__ q_out, int64_t ldo,
+                                                              uint16_t* q_out, int64_t ldo,
                                                               uint16_t* __restrict__ k_pages,
                                                               uint16_t* __restrict__ v_pages, int Hq, int Hkv,
                                                               int shift, int64_t tokens, double log2_theta, float eps) {

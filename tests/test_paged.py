@@ -183,3 +183,29 @@ def test_the_model_keeps_its_references(seed):
         m.check()
         for r in range(6):  # what a request holds has pages of its own or shared ones
             assert (m.tables[r, :-(-m.lengths[r] // 16)] >= 0).all()
+
+
+def test_paged_cache_and_decoder_refuse_before_they_reach_the_gpu():
+    from ironmule_amd.decode import DecoderConfig, random_weights
+    from ironmule_amd.paged import PagedCache, PagedDecoder
+    cfg = DecoderConfig(hidden=256, layers=1, heads=4, kv_heads=2, head_dim=128, intermediate=512, vocab=512)
+    for bad in ({"requests": 0}, {"requests": 1025}, {"capacity": 0}, {"pages": 0}, {"rows": 0}, {"page_size": 8},
+                {"page_size": 48}, {"page_size": 2048}):
+        with pytest.raises(ValueError):
+            PagedCache(cfg, **{**dict(requests=2, capacity=64, pages=8, rows=16, device="cpu"), **bad})
+    cache = PagedCache(cfg, 2, 65, 8, 16, "cpu", page_size=16)
+    assert cache.capacity == 80 and cache.tables.shape == (2, 5)
+    assert cache.pool.shape == (2, 8, 2, 16, 128)
+    for rows in (0, 17):
+        with pytest.raises(ValueError):
+            cache.reserve([1, 1], rows)
+    with pytest.raises(ValueError):  # tensors on the host
+        cache.reserve([1, 1])
+    with pytest.raises(ValueError):
+        cache.fork(0, [1])
+    weights = random_weights(cfg, "cpu")
+    with pytest.raises(ValueError):
+        PagedDecoder(weights, PagedCache(DecoderConfig(), 1, 16, 1, 1, "cpu"))
+    small = DecoderConfig(hidden=256, layers=1, heads=4, kv_heads=2, head_dim=64, intermediate=512, vocab=512)
+    with pytest.raises(ValueError):
+        PagedDecoder(random_weights(small, "cpu"), PagedCache(small, 1, 16, 1, 1, "cpu"))
