@@ -1053,6 +1053,7 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
 // the longest context has kTileAlone keys or fewer.
 constexpr int kTile = 128, kTileLeast = 256, kTileAlone = 1024;  // (keys)
 constexpr float kSlack = 8.0f;
+constexpr int kAhead = 4, kAheadV = 4;  // operands of K and of V^T that are in registers or on their way there
 
 template <int D>
 constexpr int tile_block() {
@@ -1151,21 +1152,28 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
   float top = -INFINITY, sum = 0.0f;  // (in units of raw scores times scale_log2)
 
   if (from < stop) {
-    const scalar_ints table = (scalar_ints)(a.tables + (int64_t)s.request * a.columns);
+    const int32_t* const table = a.tables + (int64_t)s.request * a.columns;
     const int mask = (1 << a.shift) - 1;
+    // The pages of 64 groups of 16 keys, one a lane, and of the 64 after those: loaded long before they are
+    // used.  (A scalar load for each block cost its whole latency: LDS reads wait for scalar loads too.)
+    constexpr int AHEAD = 64 / GROUPS;  // blocks
+    auto read_pages = [&](int block) __attribute__((always_inline)) {
+      return table[min(block * KEYS + 16 * lane, tile_last) >> a.shift];
+    };
+    int seen = from, pages_now = read_pages(from), pages_next = read_pages(from + AHEAD);
     // Of a block: the page of this wavefront's keys (a bad one read as page 0), and which 16-key groups have a
     // bad page.
     auto look_up = [&](int block, int* page, uint32_t* bad) __attribute__((always_inline)) {
       block = min(block, stop - 1);
-      *page = 0;
-      *bad = 0;
-#pragma unroll
-      for (int b = 0; b < GROUPS; ++b) {
-        const int p = table[min(block * KEYS + 16 * b, tile_last) >> a.shift];
-        const bool held = (uint32_t)p < (uint32_t)a.pages;
-        *bad |= held ? 0u : 1u << b;
-        *page = held && wave * MINE / 16 == b ? p : *page;
+      if (block - seen >= AHEAD) {
+        seen += AHEAD;
+        pages_now = pages_next;
+        pages_next = read_pages(seen + AHEAD);
       }
+      const int at = (block - seen) * GROUPS;
+      const int p = __builtin_amdgcn_readlane(pages_now, at + wave * MINE / 16);
+      *page = (uint32_t)p < (uint32_t)a.pages ? p : 0;
+      *bad = (uint32_t)(__ballot((uint32_t)pages_now >= (uint32_t)a.pages) >> at) & ((1u << GROUPS) - 1);
     };
     // Memory -> LDS, 1 KB a load: lane l gets the 16 bytes at l.  The swizzle is in where the lane reads: of
     // row r it takes the piece that belongs in its place.  A wavefront's MINE keys lie in one page.
@@ -1199,12 +1207,39 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
         sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, w), qf[t], t ? sc[b] : f32x16_t{}, 0, 0, 0);
       }
     };
-    // One block: its scores in sc, its values in vb; the next one's keys are in kb, and its scores
-    // replace this one's.  The keys after that go to k_free, the next values to v_free.
-    f32x16_t sc[B];
+    // K and V as the matrix instructions take them: of K the keys 32 b .. + 31 and dimensions 16 t .. + 15
+    // (j = B t + b), of V^T the dimensions 32 c .. + 31 and keys 16 u .. + 15 (j = C u + c)
+    auto key_operand = [&](const char* kb, uint32_t at, int j) __attribute__((always_inline)) {
+      return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const u32x4_t*>(kb + 32 * (j % B) * 2 * D + (at ^ (32 * (j / B)))));
+    };
+    uint32_t v_lane[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * h + ((lane & 15) >> 2);
+      v_lane[i] = r * 2 * D + 64 * (i ^ (r & 3)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    }
+    auto value_operand = [&](const char* vb, int j) __attribute__((always_inline)) {
+      const char* const at = vb + v_lane[j % C % 4] + 64 * (j % C / 4 * 4) + 16 * (j / C) * 2 * D;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * 2 * D));
+      return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto highest = [&](const f32x16_t* sc) __attribute__((always_inline)) {  // (a NaN score comes back through its exponential)
+      float most = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) most = fmaxf(most, sc[b][i]);
+      return most;
+    };
+    // One block: its scores in sc, its values in vb; the next one's keys are in kb, its scores become
+    // `ahead`.  The keys after that go to k_free, the next values to v_free.
+    f32x16_t scores0[B], scores1[B];
+    float most;                      // of the block's scores
     int page1, page2;                // the next block's page, and the one's after that
     uint32_t bad0, bad1, bad2;       // this block's bad groups, and those of the two
-    auto turn = [&](int block, const char* kb, char* k_free, char* vb, char* v_free) __attribute__((always_inline)) {
+    auto turn = [&](int block, f32x16_t* sc, f32x16_t* ahead, const char* kb, char* k_free, char* vb,
+                    char* v_free) __attribute__((always_inline)) {
       // this wavefront's part of the next keys and of these values has landed; past the barrier every
       // wavefront's has, and nobody reads the free arrays
       wait_vmem();
@@ -1240,12 +1275,8 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
             const bool seen = !((bad0 >> (2 * b + (i >> 3))) & 1) & (key <= p) & (key > first);
             sc[b][i] = seen ? sc[b][i] : -INFINITY;
           }
+        most = highest(sc);
       }
-      float most = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < B; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) most = fmaxf(most, sc[b][i]);  // (a NaN score comes back through its exponential)
       most = max_xor32(most) * a.scale_log2;
       if (__any(most > top + kSlack)) {
         const float higher = fmaxf(most, top), base = higher == -INFINITY ? 0.0f : higher;
@@ -1256,26 +1287,47 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
         for (int c = 0; c < C; ++c) o[c] *= keep;
       }
       const float base = top == -INFINITY ? 0.0f : top;
-      // the next block's scores, and between their MFMAs this one's probabilities
-      f32x16_t ahead[B];
+      // The next block's scores, and this one's probabilities between them; then the values, and the next
+      // block's maximum between them.  A wavefront issues in order: each matrix instruction here is followed
+      // by the reads for one a few later and by as much arithmetic as fits under it.  REPLACE_PIPE
+      constexpr int N = T * B, M = C * KEYS / 16, PAIRS = 8 * B;  // matrix instructions of either kind
       uint32_t k_at = k_lane;
       asm volatile("" : "+v"(k_at));  // (one register, and an instruction for each read's address)
       u32x4_t pw[KEYS / 16];
+      bf16x8_t kf[kAhead], vf[kAheadV];
 #pragma unroll
-      for (int t = 0; t < T; ++t) scores(kb, k_at, t, ahead);
+      for (int j = 0; j < kAhead - 1; ++j) kf[j] = key_operand(kb, k_at, j);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int b = 0; b < B; ++b)
+      for (int j = 0; j < N; ++j) {
+        if (j + kAhead - 1 < N) kf[(j + kAhead - 1) % kAhead] = key_operand(kb, k_at, j + kAhead - 1);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sc[b][i] = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.scale_log2, -base));
-          sum += sc[b][i];
+        for (int i = 0; i < kAheadV; ++i)
+          if (j == N - kAheadV / 2 + i / 2) vf[i] = value_operand(vb, i);
+        ahead[j % B] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % kAhead], qf[j / B], j < B ? f32x16_t{} : ahead[j % B], 0, 0, 0);
+#pragma unroll
+        for (int e = j * PAIRS / N; e < (j + 1) * PAIRS / N; ++e) {
+          const int b = e / 8, i = 2 * (e % 8);
+          const float lo = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.scale_log2, -base));
+          const float hi = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], a.scale_log2, -base));
+          sum += lo;
+          sum += hi;
+          pw[2 * b + i / 8][i / 2 % 4] = pack_bf16(lo, hi);
         }
-#pragma unroll
-      for (int u = 0; u < KEYS / 16; ++u) {
-        const int b = u >> 1, i0 = 8 * (u & 1);
-        pw[u] = u32x4_t{pack_bf16(sc[b][i0], sc[b][i0 + 1]), pack_bf16(sc[b][i0 + 2], sc[b][i0 + 3]),
-                        pack_bf16(sc[b][i0 + 4], sc[b][i0 + 5]), pack_bf16(sc[b][i0 + 6], sc[b][i0 + 7])};
+        __builtin_amdgcn_sched_barrier(0);
       }
+      most = -INFINITY;  // (a NaN score comes back through its exponential)
+#pragma unroll
+      for (int j = 0; j < M; ++j) {
+        o[j % C] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j % kAheadV], __builtin_bit_cast(bf16x8_t, pw[j / C]), o[j % C], 0, 0, 0);
+        if (j + kAheadV < M) vf[j % kAheadV] = value_operand(vb, j + kAheadV);
+        if (j >= 4) {
+#pragma unroll
+          for (int e = (j - 4) * 16 * B / (M - 4); e < (j - 3) * 16 * B / (M - 4); ++e) most = fmaxf(most, ahead[e / 16][e % 16]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      asm volatile("" : "+v"(most));  // (worked out here, not where it is used)
       if (odd) {
         int l = lane, p = live ? position : -1;
         asm volatile("" : "+v"(l), "+v"(p));
@@ -1283,11 +1335,10 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
           const int key = k0 + r;
           if (((bad0 >> (r >> 4)) & 1) || key < low || key > tile_last) continue;
           const int which = 16 * (r >> 5) + 4 * ((r >> 3) & 3) + (r & 3);
-          float mine = 0.0f;
+          uint32_t word = 0;
 #pragma unroll
-          for (int b = 0; b < B; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mine = which == 16 * b + i ? sc[b][i] : mine;
+          for (int e = 0; e < PAIRS; ++e) word = which >> 1 == e ? pw[e / 4][e % 4] : word;
+          const float mine = __uint_as_float(which & 1 ? word & 0xffff0000u : word << 16);
           const float pr = __shfl(mine, (l & 31) + 32 * ((r >> 2) & 1));
           const bool seen = key <= p && (!a.window || key > p - a.window);
           const uint16_t* const v = a.v_pages + ((((int64_t)table[key >> a.shift] * a.Hkv + head) << a.shift) + (key & mask)) * D;
@@ -1297,24 +1348,10 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
             for (int i = 0; i < 16; ++i) {
               const uint32_t bits = v[32 * c + 8 * (i >> 2) + 4 * (l >> 5) + (i & 3)];
               if (seen && (bits & 0x7f80u) == 0x7f80u) o[c][i] += pr * bf16_bits_to_f32(bits);
+              if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few registers: the loop above needs them)
             }
         }
       }
-#pragma unroll
-      for (int u = 0; u < KEYS / 16; ++u) {
-        const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw[u]);
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const int r = 16 * u + 4 * h + ((lane & 15) >> 2);
-          const char* const at = vb + r * 2 * D + 64 * (c ^ (r & 3)) + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-          const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)at);
-          const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 8 * 2 * D));
-          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-          o[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf, o[c], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int b = 0; b < B; ++b) sc[b] = ahead[b];
       page1 = page2;
       bad0 = bad1;
       bad1 = bad2;
@@ -1338,10 +1375,11 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int t = 0; t < T; ++t) scores(k0l, k_lane, t, sc);
+    for (int t = 0; t < T; ++t) scores(k0l, k_lane, t, scores0);
+    most = highest(scores0);
     for (int block = from; block < stop; block += 2) {
-      turn(block, k1l, k0l, v0l, v1l);
-      if (block + 1 < stop) turn(block + 1, k0l, k1l, v1l, v0l);
+      turn(block, scores0, scores1, k1l, k0l, v0l, v1l);
+      if (block + 1 < stop) turn(block + 1, scores1, scores0, k0l, k1l, v1l, v0l);
     }
     wait_vmem();  // the loads past the last block, before the LDS is given up
     sum = add_xor32(sum);
@@ -1392,10 +1430,10 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, int index, Merge
 enum { kFew = 1, kMany = 2 };
 
 __device__ __forceinline__ int own_index(int block, int few_groups, int many_groups, bool* few) {
-  const int both = min(few_groups, many_groups) & ~7;  // of either kind in turn
+  const int both = min(few_groups, many_groups) & ~31;  // of either kind in turn
   if (block < 2 * both) {
-    *few = !(block & 8);
-    return (block >> 4) * 8 + (block & 7);
+    *few = !(block & 32);
+    return (block >> 6) * 32 + (block & 31);
   }
   block -= both;
   *few = block < few_groups;
