@@ -553,7 +553,10 @@ __device__ __forceinline__ Request read_request(const AttendArgs& a, int r) {
     const int queries = q.count * a.group;
     q.tiles = queries < a.fewest || queries > a.most ? 0 : (queries + WIDTH - 1) / WIDTH;
     q.block0 = (a.window ? max(0, q.end - q.count - a.window + 1) : 0) / BLOCK;
-    q.blocks = max(1, (((q.end + BLOCK - 1) / BLOCK - q.block0) + (1 << a.grain) - 1) >> a.grain);
+    int blocks = (q.end + BLOCK - 1) / BLOCK - q.block0;
+    // (a tile of many queries goes over its own rows' windows only)
+    if (WIDTH > 16 && a.window) blocks = min(blocks, (a.window + (WIDTH - 2) / a.group) / BLOCK + 2);
+    q.blocks = max(1, (blocks + (1 << a.grain) - 1) >> a.grain);
   }
   return q;
 }
@@ -621,6 +624,18 @@ struct Line {
   }
 };
 
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+
+__device__ __forceinline__ int wave_highest(int v) {  // (of values >= 0; as wave_scan)
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+
 struct BlocksOf {
   __device__ __forceinline__ int operator()(const Request& q) const { return q.blocks; }
 };
@@ -641,6 +656,11 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t w, uint32_t* odd) {
   const bool lo = (w & 0x7f80u) == 0x7f80u, hi = (w & 0x7f800000u) == 0x7f800000u;
   *odd |= lo || hi;
   return (lo ? 0u : w & 0xffffu) | (hi ? 0u : w & 0xffff0000u);
+}
+
+typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {  // v_pk_max_u16
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, a), __builtin_bit_cast(u16x2_t, b)));
 }
 
 // Few queries per request (decode steps, short chunks): tiles of 16 queries of one KV head.  The line of
@@ -1053,6 +1073,7 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
 // the longest context has kTileAlone keys or fewer.
 constexpr int kTile = 128, kTileLeast = 256, kTileAlone = 1024;  // (keys)
 constexpr float kSlack = 8.0f;
+constexpr int kCUs = 256;
 constexpr int kAhead = 4, kAheadV = 4;  // operands of K and of V^T that are in registers or on their way there
 
 template <int D>
@@ -1073,13 +1094,46 @@ struct SplitsOf {  // a request's splits of a tile: where there is one only, or 
   }
 };
 
-// The blocks of a split.
-template <typename LANES>
+// The blocks of a split.  Three choices: whole tiles; as many splits of each as leave a CU to every one; and
+// as many as are resident.  What each costs, in blocks (about 1 us): the longest split with its start and
+// end (kStart), or what a CU has to do (with two workgroups on it they share it, and others wait for a
+// quarter of the longest; with one, heads of 256, a last round may be short); and where tiles are split, the
+// second launch and its partial results (kJoin).  512 queries of 32 heads on 8: whole over 1024 keys 27 us
+// and split 32, over 4096 keys 75 and 55.
+constexpr float kStart = 5.0f;
+template <int D>
+constexpr float kJoin = D == 128 ? 10.0f : 20.0f;
+template <int D, typename LANES>
 __device__ __forceinline__ int tile_chunk(LANES& lanes, int least) {
   const AttendArgs& a = lanes.a;
   if (a.units == 0) return 1 << 30;
-  Line<LANES, BlocksOf> work(lanes, BlocksOf());
-  return max(max(1, least >> a.grain), ceil_of(work.total, a.units));
+  least = max(1, least >> a.grain);
+  int work = 0, tiles = 0, longest = 0;
+  for (int base = 0; base < a.requests; base += 64) {
+    lanes.read(base);
+    work += wave_total(lanes.q.tiles * lanes.q.blocks);
+    tiles += wave_total(lanes.q.tiles);
+    longest = max(longest, wave_highest(lanes.q.tiles ? lanes.q.blocks : 0));
+  }
+  const int cus = max(1, kCUs / a.Hkv);
+  const auto cost = [&](int splits, int blocks) {
+    const float mean = (float)work / (float)splits + kStart;
+    const float shared = D == 128 ? mean * (float)splits / (float)cus + 0.25f * (float)blocks : mean * (float)ceil_of(splits, cus);
+    return fmaxf((float)blocks + kStart, shared);
+  };
+  const int fine = max(least, ceil_of(work, a.units));
+  if (fine >= longest) return 1 << 30;
+  const int coarse = max(fine, ceil_of(longest, max(1, cus / tiles)));
+  int splits_fine = 0, splits_coarse = 0;
+  for (int base = 0; base < a.requests; base += 64) {
+    lanes.read(base);
+    splits_fine += wave_total(lanes.q.tiles * ceil_of(lanes.q.blocks, fine));
+    splits_coarse += wave_total(lanes.q.tiles * ceil_of(lanes.q.blocks, coarse));
+  }
+  const float whole = cost(tiles, longest), with_coarse = cost(splits_coarse, min(coarse, longest)) + kJoin<D>;
+  const float with_fine = cost(splits_fine, fine) + kJoin<D>;
+  if (whole <= fminf(with_coarse, with_fine)) return 1 << 30;
+  return with_coarse < with_fine ? coarse : fine;
 }
 
 // Split number `unit`; request -1 past the last one.
@@ -1128,10 +1182,11 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
   constexpr int MINE = KEYS / 4, L = MINE * P / 64;  // keys of a block that a wavefront loads, 1 KB at a time
   constexpr int GROUPS = KEYS / 16;
   static_assert(KEYS * 2 * D == kArray, "a block's keys, or its values, fill an array");
+  __shared__ __attribute__((aligned(16))) int odd_waves[4];
   const int head = index % a.Hkv, lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Lanes<kTile, KEYS> lanes(a);
-  const int chunk = tile_chunk(lanes, kTileLeast / KEYS);
+  const int chunk = tile_chunk<D>(lanes, kTileLeast / KEYS);
   const TilePart s = find_part(lanes, index / a.Hkv, chunk);
   if (s.request < 0) return;
   int tile_first, tile_last, low, block0;
@@ -1163,13 +1218,15 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
     int seen = from, pages_now = read_pages(from), pages_next = read_pages(from + AHEAD);
     // Of a block: the page of this wavefront's keys (a bad one read as page 0), and which 16-key groups have a
     // bad page.
-    auto look_up = [&](int block, int* page, uint32_t* bad) __attribute__((always_inline)) {
-      block = min(block, stop - 1);
-      if (block - seen >= AHEAD) {
+    auto move_pages = [&](int block) __attribute__((always_inline)) {
+      if (min(block, stop - 1) - seen >= AHEAD) {
         seen += AHEAD;
         pages_now = pages_next;
         pages_next = read_pages(seen + AHEAD);
       }
+    };
+    auto look_up = [&](int block, int* page, uint32_t* bad) __attribute__((always_inline)) {  // (after move_pages)
+      block = min(block, stop - 1);
       const int at = (block - seen) * GROUPS;
       const int p = __builtin_amdgcn_readlane(pages_now, at + wave * MINE / 16);
       *page = (uint32_t)p < (uint32_t)a.pages ? p : 0;
@@ -1184,14 +1241,19 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
       k_from[i] = in * 2 * D + 16 * (piece ^ (r & 15));
       v_from[i] = in * 2 * D + 64 * ((piece >> 2) ^ (r & 3)) + 16 * (piece & 3);
     }
-    auto load = [&](const uint16_t* pages, int page, int block, const uint32_t* lane_from, char* to) __attribute__((always_inline)) {
+    auto source = [&](const uint16_t* pages, int page, int block) __attribute__((always_inline)) {
       block = min(block, stop - 1);
       const int64_t at = ((((int64_t)page * a.Hkv + head) << a.shift) + ((block * KEYS + wave * MINE) & mask)) * D;
-      const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc(pages + at, MINE * 2 * D);
+      return buffer_rsrc(pages + at, MINE * 2 * D);
+    };
+    auto load_kb = [&](__amdgpu_buffer_rsrc_t rsrc, int i, const uint32_t* lane_from, char* to) __attribute__((always_inline)) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (__attribute__((address_space(3))) void*)(to + wave * MINE * 2 * D + 1024 * i), 16, lane_from[i], 0, 0, 0);
+    };
+    auto load = [&](const uint16_t* pages, int page, int block, const uint32_t* lane_from, char* to) __attribute__((always_inline)) {
+      const __amdgpu_buffer_rsrc_t rsrc = source(pages, page, block);
 #pragma unroll
-      for (int i = 0; i < L; ++i)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rsrc, (__attribute__((address_space(3))) void*)(to + wave * MINE * 2 * D + 1024 * i), 16, lane_from[i], 0, 0, 0);
+      for (int i = 0; i < L; ++i) load_kb(rsrc, i, lane_from, to);
     };
     // Where some queries see a key of the block and others do not, or none does (see attend_rows)
     auto is_edge = [&](int block, uint32_t bad) __attribute__((always_inline)) {
@@ -1245,8 +1307,7 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
       wait_vmem();
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
-      load(a.k_pages, page2, block + 2, k_from, k_free);
-      load(a.v_pages, page1, block + 1, v_from, v_free);
+      move_pages(block + 3);
       const int k0 = KEYS * block;
       const bool edge = is_edge(block, bad0);
       int odd = 0;
@@ -1254,30 +1315,49 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
         // (what only edges need is worked out here, not kept in registers over the loop)
         int l = lane, p = position;
         asm volatile("" : "+v"(l), "+v"(p));
-        uint32_t found = 0;
+        // An infinity or a NaN among the values?  (a probability of zero must not meet one)
+        uint32_t exponents = 0;
 #pragma unroll
         for (int i = 0; i < L; ++i) {
-          const int r = wave * MINE + (64 / P) * i + l / P, key = k0 + r;
-          const bool good = !((bad0 >> (r >> 4)) & 1) && key >= low && key <= tile_last;
-          u32x4_t* const at = reinterpret_cast<u32x4_t*>(vb + wave * MINE * 2 * D + 1024 * i + 16 * l);
-          u32x4_t w = *at;
+          const u32x4_t w = *reinterpret_cast<const u32x4_t*>(vb + wave * MINE * 2 * D + 1024 * i + 16 * l);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = good ? finite_pair(w[e], &found) : 0u;
-          *at = w;
+          for (int e = 0; e < 4; ++e) exponents = max_pair(exponents, w[e] & 0x7f807f80u);
         }
-        odd = __syncthreads_or((int)found);
-        const int first = a.window ? p - a.window : -1;  // (the last key that the query no longer sees)
+        // (not __syncthreads_or, which loads the size of the workgroup)
+        const uint64_t any = __ballot((exponents & 0xffffu) == 0x7f80u || exponents >> 16 == 0x7f80u);
+        if (lane == 0) odd_waves[wave] = any != 0;
+        __syncthreads();
+        const int4 odds = *reinterpret_cast<const int4*>(odd_waves);
+        odd = odds.x | odds.y | odds.z | odds.w;
+        if (odd) {
+#pragma unroll
+          for (int i = 0; i < L; ++i) {
+            u32x4_t* const at = reinterpret_cast<u32x4_t*>(vb + wave * MINE * 2 * D + 1024 * i + 16 * l);
+            u32x4_t w = *at;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = finite_pair(w[e], &exponents);
+            *at = w;
+          }
+          __syncthreads();
+        }
+        // the query sees the keys that are less than `span` before its own
+        const int own = p - k0 - 4 * (l >> 5);
+        const uint32_t span = a.window ? a.window : 0x7fffffff;
 #pragma unroll
         for (int b = 0; b < B; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int key = k0 + 32 * b + 8 * (i >> 2) + 4 * (l >> 5) + (i & 3);
-            const bool seen = !((bad0 >> (2 * b + (i >> 3))) & 1) & (key <= p) & (key > first);
-            sc[b][i] = seen ? sc[b][i] : -INFINITY;
+            const int key = 32 * b + 8 * (i >> 2) + (i & 3);
+            sc[b][i] = (uint32_t)(own - key) < span ? sc[b][i] : -INFINITY;
           }
-        most = highest(sc);
+        if (bad0)
+#pragma unroll
+          for (int b = 0; b < B; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[b][i] = (bad0 >> (2 * b + (i >> 3))) & 1 ? -INFINITY : sc[b][i];
+        most = max_xor32(highest(sc));
       }
-      most = max_xor32(most) * a.scale_log2;
+      most *= a.scale_log2;
       if (__any(most > top + kSlack)) {
         const float higher = fmaxf(most, top), base = higher == -INFINITY ? 0.0f : higher;
         const float keep = __builtin_amdgcn_exp2f(top - base);
@@ -1295,6 +1375,19 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
       asm volatile("" : "+v"(k_at));  // (one register, and an instruction for each read's address)
       u32x4_t pw[KEYS / 16];
       bf16x8_t kf[kAhead], vf[kAheadV];
+      __amdgpu_buffer_rsrc_t k_source, v_source;
+      static_assert(2 + 2 * L <= N, "the loads have their steps");
+      auto probabilities = [&](int step) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = step * PAIRS / (N + M / 2); e < (step + 1) * PAIRS / (N + M / 2); ++e) {
+          const int b = e / 8, i = 2 * (e % 8);
+          const float lo = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.scale_log2, -base));
+          const float hi = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], a.scale_log2, -base));
+          sum += lo;
+          sum += hi;
+          pw[2 * b + i / 8][i / 2 % 4] = pack_bf16(lo, hi);
+        }
+      };
 #pragma unroll
       for (int j = 0; j < kAhead - 1; ++j) kf[j] = key_operand(kb, k_at, j);
       __builtin_amdgcn_sched_barrier(0);
@@ -1305,15 +1398,12 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
         for (int i = 0; i < kAheadV; ++i)
           if (j == N - kAheadV / 2 + i / 2) vf[i] = value_operand(vb, i);
         ahead[j % B] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[j % kAhead], qf[j / B], j < B ? f32x16_t{} : ahead[j % B], 0, 0, 0);
-#pragma unroll
-        for (int e = j * PAIRS / N; e < (j + 1) * PAIRS / N; ++e) {
-          const int b = e / 8, i = 2 * (e % 8);
-          const float lo = __builtin_amdgcn_exp2f(fmaf(sc[b][i], a.scale_log2, -base));
-          const float hi = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], a.scale_log2, -base));
-          sum += lo;
-          sum += hi;
-          pw[2 * b + i / 8][i / 2 % 4] = pack_bf16(lo, hi);
-        }
+        probabilities(j);
+        // (the next loads: their addresses, then 1 KB at a time)
+        if (j == 0) k_source = source(a.k_pages, page2, block + 2);
+        if (j == 1) v_source = source(a.v_pages, page1, block + 1);
+        if (j >= 2 && j < 2 + L) load_kb(k_source, j - 2, k_from, k_free);
+        if (j >= 2 + L && j < 2 + 2 * L) load_kb(v_source, j - 2 - L, v_from, v_free);
         __builtin_amdgcn_sched_barrier(0);
       }
       most = -INFINITY;  // (a NaN score comes back through its exponential)
@@ -1321,19 +1411,27 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
       for (int j = 0; j < M; ++j) {
         o[j % C] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[j % kAheadV], __builtin_bit_cast(bf16x8_t, pw[j / C]), o[j % C], 0, 0, 0);
         if (j + kAheadV < M) vf[j % kAheadV] = value_operand(vb, j + kAheadV);
-        if (j >= 4) {
+        if (j < M / 2) {
+          probabilities(N + j);
+        } else {
 #pragma unroll
-          for (int e = (j - 4) * 16 * B / (M - 4); e < (j - 3) * 16 * B / (M - 4); ++e) most = fmaxf(most, ahead[e / 16][e % 16]);
+          for (int e = (2 * j - M) * 16 * B / M; e < (2 * j + 2 - M) * 16 * B / M; ++e) most = fmaxf(most, ahead[e / 16][e % 16]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+      most = max_xor32(most);
       asm volatile("" : "+v"(most));  // (worked out here, not where it is used)
+      const uint32_t bad = bad0;
+      page1 = page2;
+      bad0 = bad1;
+      bad1 = bad2;
+      look_up(block + 3, &page2, &bad2);
       if (odd) {
         int l = lane, p = live ? position : -1;
         asm volatile("" : "+v"(l), "+v"(p));
         for (int r = 0; r < KEYS; ++r) {
           const int key = k0 + r;
-          if (((bad0 >> (r >> 4)) & 1) || key < low || key > tile_last) continue;
+          if (((bad >> (r >> 4)) & 1) || key < low || key > tile_last) continue;
           const int which = 16 * (r >> 5) + 4 * ((r >> 3) & 3) + (r & 3);
           uint32_t word = 0;
 #pragma unroll
@@ -1352,10 +1450,6 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
             }
         }
       }
-      page1 = page2;
-      bad0 = bad1;
-      bad1 = bad2;
-      look_up(block + 3, &page2, &bad2);
     };
 
     int page0;
@@ -1376,7 +1470,7 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < T; ++t) scores(k0l, k_lane, t, scores0);
-    most = highest(scores0);
+    most = max_xor32(highest(scores0));
     for (int block = from; block < stop; block += 2) {
       turn(block, scores0, scores1, k1l, k0l, v0l, v1l);
       if (block + 1 < stop) turn(block + 1, scores1, scores0, k0l, k1l, v1l, v0l);
@@ -1413,7 +1507,7 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, int index, Merge
   constexpr int KEYS = tile_block<D>();
   const int head = index % a.Hkv;
   Lanes<kTile, KEYS> lanes(a);
-  const int chunk = tile_chunk(lanes, kTileLeast / KEYS);
+  const int chunk = tile_chunk<D>(lanes, kTileLeast / KEYS);
   const TilePart s = find_part(lanes, index / a.Hkv, chunk);
   if (s.request < 0 || s.splits == 1) return;
   int tile_first, tile_last, low, block0;
