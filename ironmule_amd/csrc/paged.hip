@@ -1055,22 +1055,25 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
 }
 
 // Many queries per request (chunks of prompts): tiles of 128 queries of one KV head, each of a workgroup's
-// four wavefronts 32 of them; the key blocks go through LDS, shared by the four
-// and twice there, the next block's loads in flight in registers over the current one's work and one
-// barrier per block.  Scores are K Q^T on v_mfma_f32_32x32x16_bf16 and P^T the B operand of V^T P^T without
-// leaving its lane, as above (keys 4 h .. and 8 + 4 h .. of 16).  The running maximum follows only when
-// a score passes it by 2^8: until then the probabilities are up to 256, which costs no accuracy, and the
-// sums need not be scaled again.  K lies in LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both
-// swizzled so that the rows that a read takes at a time lie in different banks (the 32-byte pieces of
-// attend_rows and K's by row & 7 had every read conflict once: half of the LDS cycles).
+// four wavefronts 32 of them; the key blocks go through LDS, shared by the four and twice there, the loads
+// of the next one in flight over the current one's work and one barrier per block.  Scores are K Q^T on
+// v_mfma_f32_32x32x16_bf16 and P^T the B operand of V^T P^T without leaving its lane, as above (keys 4 h ..
+// and 8 + 4 h .. of 16).  The running maximum follows only when a score passes it by 2^8: until then the
+// probabilities are up to 256, which costs no accuracy, and the sums need not be scaled again.  K lies in
+// LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both swizzled so that the rows that a read takes
+// at a time lie in different banks (the 32-byte pieces of attend_rows and K's by row & 7 had every read
+// conflict once: half of the LDS cycles).
 //
-// A tile is cut into splits of at most `chunk` blocks, the chunk such that there are about as many
-// as workgroups are resident.  Tiles of requests that have several splits come first, and a request's last tiles, the longest,
-// before its first ones.
+// A tile is cut into splits of at most `chunk` blocks (tile_chunk).  Tiles of requests that have several
+// splits come first, and a request's last tiles, the longest, before its first ones.
 //
-// A block takes a workgroup alone on its CU 0.7 us, two of them 1.45 together; a launch's start, the first
-// block with its instructions still to be fetched, and its end 8, the second launch 5.  So no tile is split where
-// the longest context has kTileAlone keys or fewer.
+// Bound by the matrix cores' power and by what a wavefront can issue between their instructions: 8192 tokens
+// of 32 heads of 128 in 515 to 530 us (1040 to 1070 TFLOP/s; a library product of 8192^3 reaches 1200), where the
+// cores are busy 54 % of the time at 1.8 GHz.  A block takes 1.0 us (heads of 256) or 1.1 (128) alone on a CU and
+// two workgroups there do one each in 2.1; an edge takes 0.5 us more; a workgroup's start and end take 5 us,
+// the second launch 5 and its partial results' traffic.  So no tile is split where the longest context has
+// kTileAlone keys, or twice that and there are tiles for a quarter of the CUs (512 queries of 32 heads over
+// 1024 keys 24 us, 28 with a second launch).
 constexpr int kTile = 128, kTileLeast = 256, kTileAlone = 1024;  // (keys)
 constexpr float kSlack = 8.0f;
 constexpr int kCUs = 256;
@@ -1369,7 +1372,8 @@ __device__ __forceinline__ void tile_workgroup(const AttendArgs& a, int index, c
       const float base = top == -INFINITY ? 0.0f : top;
       // The next block's scores, and this one's probabilities between them; then the values, and the next
       // block's maximum between them.  A wavefront issues in order: each matrix instruction here is followed
-      // by the reads for one a few later and by as much arithmetic as fits under it.  REPLACE_PIPE
+      // by the reads for one a few later and by as much arithmetic as fits under it.  Left to the
+      // compiler, which read each operand just before its instruction: 8192 tokens 576 us, now 523.
       constexpr int N = T * B, M = C * KEYS / 16, PAIRS = 8 * B;  // matrix instructions of either kind
       uint32_t k_at = k_lane;
       asm volatile("" : "+v"(k_at));  // (one register, and an instruction for each read's address)
@@ -1519,8 +1523,10 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, int index, Merge
 }
 
 // A launch for requests of few queries, of many, or of both: `few_groups` and `many_groups` workgroups.
-// With both, eight of one kind and eight of the other in turn (an XCD gets workgroups of both), so that those that
-// wait for memory and those that multiply share the CUs: the mixed batch of 24 in 138 us one after the other.
+// With both, 32 of one kind and 32 of the other in turn (every shader engine gets workgroups of both), so that those that
+// wait for memory and those that multiply share the CUs: a mixed batch of 24 requests in 87 us, 102 one kind
+// after the other.  (In turns of eight, one workgroup of each kind per XCD, half of an XCD's shader engines got all of the
+// tiles: 103.)
 enum { kFew = 1, kMany = 2 };
 
 __device__ __forceinline__ int own_index(int block, int few_groups, int many_groups, bool* few) {
@@ -1652,7 +1658,9 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
     const int keys_of = head_dim == 128 ? tile_block<128>() : tile_block<256>();
     // the chunk is the work over the units and a tile has its blocks over the chunk, rounded up, of splits: no more
     // than the units and the tiles together
-    const int64_t splits = keys <= kTileAlone ? 1 : ceil_div(keys / keys_of + 2, kTileLeast / keys_of);
+    const int64_t sure = (queries - (some_few ? kRowsMost * with : 0)) / kTile;  // tiles that there are at least
+    const bool whole = keys <= kTileAlone || (keys <= 2 * kTileAlone && 4 * sure * Hkv >= kCUs);
+    const int64_t splits = whole ? 1 : ceil_div(keys / keys_of + 2, kTileLeast / keys_of);
     l.workgroups = std::min(ceil_div(resident, Hkv) + l.tiles, l.tiles * splits);
     l.units = l.workgroups - l.tiles;
     l.slots = std::min(l.workgroups, 2 * l.units);
