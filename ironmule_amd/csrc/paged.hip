@@ -1821,6 +1821,7 @@ int32_t imq_paged_attention(const uint16_t* q, int64_t ldq, const uint16_t* k_pa
   for (const void* p : {(const void*)q, (const void*)k_pages, (const void*)v_pages, (const void*)out})
     if (!p || !aligned(p, 16)) return fail(IMQ_EINVAL, "rows and pages must be non-null and 16-byte aligned");
   if (!current_device(&code)) return code;
+  if (window >= (int64_t)columns * page_size) window = 0;  // (all that there can be: up to 2^30, so that sums of it stay in range)
   const AttendPlan plan = plan_attend(rows, requests, Hq, Hkv, head_dim,
                                       std::min<int64_t>(max_context, (int64_t)columns * page_size), window);
   const size_t nbytes = attend_space(plan.few, Hkv, head_dim) + attend_space(plan.many, Hkv, head_dim);

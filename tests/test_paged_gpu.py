@@ -332,6 +332,28 @@ def test_long_and_wide_batches_against_64_bits(env, requests, heads, kv_heads, d
     _Batch(torch, requests, heads, kv_heads, dim, page, seed=5, extra=extra).check(torch, n_, window)
 
 
+@pytest.mark.parametrize("requests,heads,kv_heads,dim,page,window", [
+    # tiles whole, cut for every CU, cut for all that are resident; many of them, few of them, other kinds between
+    ([(700, 3000), (220, 1500), (1, 2000)], 16, 8, 256, 16, 512), ([(300, 2500), (300, 2500)], 32, 8, 128, 16, 900),
+    ([(512, 2000)], 32, 8, 128, 64, 0), ([(512, 2100)], 32, 8, 128, 64, 0), ([(130, 4100)], 8, 2, 256, 32, 0),
+    ([(40, 300)] * 70 + [(1, 900)] * 3, 8, 2, 128, 32, 0), ([(70, 1300 + 10 * i) for i in range(66)], 4, 4, 128, 16, 700),
+    ([(33, 5000), (129, 129), (9, 2000)], 32, 1, 128, 16, 0), ([(65, 2048), (1, 2048)], 16, 8, 256, 128, 2000)])
+def test_tiles_however_they_are_cut_against_64_bits(env, requests, heads, kv_heads, dim, page, window):
+    torch, n_ = env
+    announce("paged attention, tiles", len(requests), requests[0], heads, kv_heads, dim, page, window)
+    _Batch(torch, requests, heads, kv_heads, dim, page, seed=6).check(torch, n_, window)
+
+
+@pytest.mark.parametrize("dim", [128, 256])
+def test_a_window_that_holds_everything_is_none(env, dim):
+    torch, n_ = env
+    announce("paged attention, wide windows", dim)
+    b = _Batch(torch, [(1, 700), (200, 500), (40, 40)], 8, 2, dim, 16, seed=9)
+    want = b.check(torch, n_).clone()
+    for window in (b.tables.shape[1] * 16, 1 << 30, 2**31 - 1):
+        assert torch.equal(b.check(torch, n_, window), want), window
+
+
 def test_bounds_on_the_context_change_nothing(env):
     torch, n_ = env
     announce("paged attention, max_context")
