@@ -720,7 +720,9 @@ def _current_gpu(*tensors: torch.Tensor) -> int:
         raise ValueError("the tensors must be on a GPU")
     if index != torch._C._cuda_getDevice():
         raise ValueError(f"the tensors are on GPU {index}, which is not the current one")
-    _same_device(index, *tensors)
+    for t in tensors:
+        if t.get_device() != index:
+            _same_device(index, t)
     return index
 
 
@@ -732,12 +734,11 @@ def _ints(name: str, t: torch.Tensor, *shape: int) -> None:
 def _cache_desc(tables, lengths, refs, page_size: int) -> PagedCacheDesc:
     if tables.dim() != 2 or refs.dim() != 1:
         raise ValueError("tables must be (requests, columns), refs (pages,)")
-    requests, columns = tables.shape
+    (requests, columns), (pages,) = tables.shape, refs.shape
     _ints("tables", tables, requests, columns)
     _ints("lengths", lengths, requests)
-    _ints("refs", refs, refs.shape[0])
-    return PagedCacheDesc(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), requests, columns, refs.shape[0],
-                          page_size)
+    _ints("refs", refs, pages)
+    return PagedCacheDesc(tables.data_ptr(), lengths.data_ptr(), refs.data_ptr(), requests, columns, pages, page_size)
 
 
 def _head_rows(name: str, t: torch.Tensor) -> int:
@@ -745,6 +746,8 @@ def _head_rows(name: str, t: torch.Tensor) -> int:
     if t.dtype is not torch.bfloat16 or t.dim() != 3:
         raise ValueError(f"{name} must be (rows, heads, head_dim) bf16, got {t.dtype} {tuple(t.shape)}")
     rows, heads, dim = t.shape
+    if dim % 8 == 0 and t.is_contiguous() and not t.is_neg():
+        return heads * dim
     across, head, one = t.stride()
     if rows <= 1:
         across = heads * dim
@@ -772,25 +775,32 @@ def paged_reserve(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tenso
     request stops sharing are copied in it.  status[r]: 0 taken, 1 no pages, 2 malformed, 3 no rows."""
     desc = _cache_desc(tables, lengths, refs, page_size)
     requests, rows = desc.requests, positions.shape[0] if positions.dim() == 1 else -1
-    _ints("counts", counts, requests)
-    _ints("starts", starts, requests + 1)
-    _ints("ends", ends, requests)
-    _ints("status", status, requests)
-    _ints("positions", positions, rows)
-    _ints("slots", slots, rows)
-    _ints("copies", copies, requests, 2)
-    _current_gpu(tables, lengths, refs, counts, starts, ends, status, positions, slots, copies)
+    i32, one, per_row = torch.int32, (requests,), (rows,)
+    if not (counts.dtype is i32 and ends.dtype is i32 and status.dtype is i32 and starts.dtype is i32
+            and positions.dtype is i32 and slots.dtype is i32 and copies.dtype is i32
+            and counts.shape == one and ends.shape == one and status.shape == one and starts.shape == (requests + 1,)
+            and positions.shape == per_row and slots.shape == per_row and copies.shape == (requests, 2)
+            and counts.is_contiguous() and ends.is_contiguous() and status.is_contiguous() and starts.is_contiguous()
+            and positions.is_contiguous() and slots.is_contiguous() and copies.is_contiguous()):
+        _ints("counts", counts, requests)  # (which of them, and the message)
+        _ints("starts", starts, requests + 1)
+        _ints("ends", ends, requests)
+        _ints("status", status, requests)
+        _ints("positions", positions, rows)
+        _ints("slots", slots, rows)
+        _ints("copies", copies, requests, 2)
+    index = _current_gpu(tables, lengths, refs, counts, starts, ends, status, positions, slots, copies)
     planes = page_bytes = address = 0
     if pool is not None:
         if pool.dim() < 3 or pool.shape[1] != desc.pages or not pool.is_contiguous():
             raise ValueError(f"the pool must be a contiguous (planes, {desc.pages}, ...) tensor")
-        _same_device(tables.get_device(), pool)
+        _same_device(index, pool)
         planes, page_bytes = pool.shape[0], pool.stride(1) * pool.element_size()
         address = pool.data_ptr()
     chunk = PagedChunkDesc(starts.data_ptr(), ends.data_ptr(), status.data_ptr(), positions.data_ptr(), slots.data_ptr(),
                            copies.data_ptr(), rows)
     _check((_lib or lib()).imq_paged_reserve(ctypes.byref(desc), counts.data_ptr(), ctypes.byref(chunk), address, planes,
-                                             page_bytes, _stream(None)))
+                                             page_bytes, torch._C._cuda_getCurrentRawStream(index)))
 
 
 def paged_reorder(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, parents: torch.Tensor,
@@ -799,8 +809,9 @@ def paged_reorder(tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tenso
     (imq_paged_reorder), on the current stream.  Forks, beams' reordering, the end of requests."""
     desc = _cache_desc(tables, lengths, refs, page_size)
     _ints("parents", parents, desc.requests)
-    _current_gpu(tables, lengths, refs, parents)
-    _check((_lib or lib()).imq_paged_reorder(ctypes.byref(desc), parents.data_ptr(), _stream(None)))
+    index = _current_gpu(tables, lengths, refs, parents)
+    _check((_lib or lib()).imq_paged_reorder(ctypes.byref(desc), parents.data_ptr(),
+                                             torch._C._cuda_getCurrentRawStream(index)))
 
 
 def paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: torch.Tensor, k_norm: torch.Tensor,
@@ -810,7 +821,7 @@ def paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: torch
     head_dim) to q_out (may be q itself), k and v (rows, kv_heads, head_dim) to the pages at `slots`; rows
     whose slot is outside the pages are left out.  Rows may lie apart (a slice of a wider projection)."""
     pages, kv_heads, page_size, dim = _pages_shape(k_pages, v_pages)
-    ldq, ldk, ldv, ldo = (_head_rows(*x) for x in (("q", q), ("k", k), ("v", v), ("q_out", q_out)))
+    ldq, ldk, ldv, ldo = _head_rows("q", q), _head_rows("k", k), _head_rows("v", v), _head_rows("q_out", q_out)
     rows, heads, _ = q.shape
     if q.shape != q_out.shape or q.shape[2] != dim or k.shape != (rows, kv_heads, dim) or v.shape != k.shape:
         raise ValueError("q and q_out must agree, k and v be (rows, kv_heads, head_dim) of the pages")
@@ -819,11 +830,11 @@ def paged_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_norm: torch
             raise ValueError(f"a norm weight must have {dim} bf16 values")
     _ints("positions", positions, rows)
     _ints("slots", slots, rows)
-    _current_gpu(q, k, v, q_norm, k_norm, positions, slots, q_out, k_pages, v_pages)
+    index = _current_gpu(q, k, v, q_norm, k_norm, positions, slots, q_out, k_pages, v_pages)
     _check((_lib or lib()).imq_paged_write(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, q_norm.data_ptr(),
                                            k_norm.data_ptr(), positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
                                            ldo, k_pages.data_ptr(), v_pages.data_ptr(), rows, heads, kv_heads, dim, pages,
-                                           page_size, theta, eps, _stream(None)))
+                                           page_size, theta, eps, torch._C._cuda_getCurrentRawStream(index)))
     return q_out
 
 
@@ -845,7 +856,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _ints("tables", tables, requests, columns)
     _ints("starts", starts, requests + 1)
     _ints("ends", ends, requests)
-    _current_gpu(q, k_pages, v_pages, tables, starts, ends, out)
+    index = _current_gpu(q, k_pages, v_pages, tables, starts, ends, out)
     library = _lib or lib()
     context = columns * page_size if max_context is None else max_context
     nbytes = library.imq_paged_attention_workspace(rows, requests, heads, kv_heads, dim, context, window)
@@ -853,7 +864,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _check(library.imq_paged_attention(q.data_ptr(), ldq, k_pages.data_ptr(), v_pages.data_ptr(), tables.data_ptr(),
                                        starts.data_ptr(), ends.data_ptr(), out.data_ptr(), ldo, rows, requests, columns,
                                        pages, page_size, heads, kv_heads, dim, context, window, scale,
-                                       ws.data_ptr() if nbytes else None, nbytes, _stream(None)))
+                                       ws.data_ptr() if nbytes else None, nbytes,
+                                       torch._C._cuda_getCurrentRawStream(index)))
     return out
 
 
@@ -873,10 +885,10 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
         raise ValueError(f"{rows} rows of logits are not groups of {beams} beams")
     if scores.dtype is not torch.float32 or scores.shape != (rows,) or not scores.is_contiguous() or scores.is_neg():
         raise ValueError(f"scores must be ({rows},) fp32")
-    _current_gpu(logits, scores)
+    index = _current_gpu(logits, scores)
     if finished is not None:
         _ints("finished", finished, rows)
-        _same_device(logits.get_device(), finished)
+        _same_device(index, finished)
     groups, library = rows // beams, _lib or lib()
     nbytes = library.imq_beam_select_workspace(groups, beams, vocab, count)
     if nbytes == 0:
@@ -888,7 +900,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, count: i
     _check(library.imq_beam_select(logits.data_ptr(), ld, _DTYPE_CODE[logits.dtype], scores.data_ptr(),
                                    finished.data_ptr() if finished is not None else None, eos, groups, beams, vocab, count,
                                    best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ended.data_ptr(),
-                                   ws.data_ptr(), nbytes, _stream(None)))
+                                   ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(index)))
     return best, parents, tokens, ended
 
 

@@ -417,7 +417,7 @@ __global__ __launch_bounds__(kMaxRequests) void reorder_lengths_kernel(int32_t* 
 // bytes.  The first heads' loads are in flight while the row's angles are computed (in double: positions
 // are large, and the angle is the product).  Two roundings to bf16, as imq_qk_norm_rope: the norm's result
 // (what the model's norm gives) and the turned value.
-// Bound by memory: 4099 rows of 48 heads of 128 (134 MB read and written) in 22.5 us, 6.0 TB/s; single
+// Bound by memory: 4099 rows of 32 heads of 256 (134 MB read and written) in 22.5 us, 6.0 TB/s; single
 // 2-byte values a lane took 34.  The slot is looked at after the loads: before them, 32.  256 to 512
 // threads are alike there, 320 and more best for a few rows (five rows 3.8 us, 4.2 with 256); a number of
 // threads by the row's heads 26.
@@ -1522,35 +1522,23 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, int index, Merge
   merge_part<kTile, D>(a, s.q, s.place, head, s.split, splits, splits, [&](int i) { return slot + i; }, space);
 }
 
-// A launch for requests of few queries, of many, or of both: `few_groups` and `many_groups` workgroups.
-// With both, 32 of one kind and 32 of the other in turn (every shader engine gets workgroups of both), so that those that
-// wait for memory and those that multiply share the CUs: a mixed batch of 24 requests in 87 us, 102 one kind
-// after the other.  (In turns of eight, one workgroup of each kind per XCD, half of an XCD's shader engines got all of the
-// tiles: 103.)
+// A launch for requests of few queries, of many, or of both: `few_groups` and `many_groups` workgroups, those
+// of many first: they are the longest, and the others, which wait for memory, share the CUs with the
+// last of them.  A mixed batch of 24 requests in 87 us, 93 in turns of 32 and 102 the other way round.  (In turns
+// of eight, one workgroup of each kind per XCD, half of an XCD's shader engines got all of the tiles: 144
+// against 117 in turns of 32.)
 enum { kFew = 1, kMany = 2 };
 
-__device__ __forceinline__ int own_index(int block, int few_groups, int many_groups, bool* few) {
-  const int both = min(few_groups, many_groups) & ~31;  // of either kind in turn
-  if (block < 2 * both) {
-    *few = !(block & 32);
-    return (block >> 6) * 32 + (block & 31);
-  }
-  block -= both;
-  *few = block < few_groups;
-  return *few ? block : block - few_groups + both;
-}
-
 template <int D, int KINDS>
-__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_kernel(AttendArgs few, AttendArgs many, int few_groups,
-                                                                            int many_groups) {
+__global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_kernel(AttendArgs few, AttendArgs many, int many_groups) {
   __shared__ __attribute__((aligned(16))) char lds0[kArray], lds1[kArray];
   __shared__ float tops[4][16], sums[4][16];
   if (KINDS == kFew && D == 128) {
     rows_workgroup<D>(few, blockIdx.x, lds0, lds1, nullptr, nullptr, tops, sums);
   } else {
     __shared__ __attribute__((aligned(16))) char lds2[kArray], lds3[kArray];
-    bool is_few = KINDS == kFew;
-    const int index = KINDS == (kFew | kMany) ? own_index(blockIdx.x, few_groups, many_groups, &is_few) : blockIdx.x;
+    const bool is_few = KINDS == kFew || (KINDS == (kFew | kMany) && (int)blockIdx.x >= many_groups);
+    const int index = KINDS == (kFew | kMany) && is_few ? blockIdx.x - many_groups : blockIdx.x;
     if ((KINDS & kFew) && is_few)
       rows_workgroup<D>(few, index, lds0, lds1, lds2, lds3, tops, sums);
     else if (KINDS & kMany)
@@ -1701,7 +1689,7 @@ void launch_attend(const AttendPlan& p, char* space, const AttendArgs& args, hip
   const auto kernel = !p.many.width  ? attend_kernel<D, kFew>
                       : !p.few.width ? attend_kernel<D, kMany>
                                      : attend_kernel<D, (kFew | kMany)>;
-  hipLaunchKernelGGL(kernel, dim3(few_groups + many_groups), dim3(kThreads), 0, stream, few, many, few_groups, many_groups);
+  hipLaunchKernelGGL(kernel, dim3(few_groups + many_groups), dim3(kThreads), 0, stream, few, many, many_groups);
   const int few_merges = p.few.slots ? (int)(p.few.units - 1) * args.Hkv : 0, many_merges = (int)p.many.slots * args.Hkv;
   if (few_merges + many_merges)
     hipLaunchKernelGGL(merge_kernel<D>, dim3(few_merges + many_merges), dim3(kThreads), 0, stream, few, many, few_merges);
