@@ -77,8 +77,10 @@ __device__ __forceinline__ void wave_fence() {
 // e-th; `some`: kSome + kRankStep places of LDS.
 //
 // The last of best[], where it is full, or else the count-th largest of the lanes' own largest values bounds
-// the count-th largest of all from below; of the latter the upper 16 bits come from 16 ballots.  Few values pass it: they are gathered in LDS, cut down to
-// those that the exact bound passes if they are over 64, and for each the better ones are counted.  Where more than kSome pass (many equal values), the best is taken count times.
+// the count-th largest of all from below; of the latter the upper 16 bits come from 16 ballots.  Few values pass
+// it: they are gathered in LDS, cut down to
+// those that the exact bound passes if they are over 64, and for each the better ones are counted.  Where more
+// than kSome pass (many equal values), the best is taken count times.
 // (Taken count times always, workgroup by workgroup: 61 us where this takes 11, for eight of each of 32 rows of
 // 262144 bf16 values.)
 template <int E, typename TOKEN>
