@@ -87,16 +87,20 @@ class PagedCache:
 
     def release(self, requests=None) -> None:
         """Ends these requests (default: all): their pages are free, or left to who shares them."""
-        parents = list(range(self.requests))
-        for r in range(self.requests) if requests is None else requests:
-            parents[r] = -1
-        self.reorder(parents)
+        self._reparent(range(self.requests) if requests is None else requests, -1)
 
     def fork(self, source: int, targets) -> None:
         """The requests `targets` become copies of request `source`."""
+        if not 0 <= source < self.requests:
+            raise ValueError(f"request {source} is not one of {self.requests}")
+        self._reparent(targets, source)
+
+    def _reparent(self, requests, parent: int) -> None:
         parents = list(range(self.requests))
-        for r in targets:
-            parents[r] = source
+        for r in requests:
+            if not 0 <= r < self.requests:
+                raise ValueError(f"request {r} is not one of {self.requests}")
+            parents[r] = parent
         self.reorder(parents)
 
 
@@ -156,16 +160,21 @@ class PagedDecoder:
 
         tokens: lists of numbers per request, or an int32 tensor (requests, width) on the GPU with counts
         there too; then `rows` bounds the sum of the counts (default: the cache's rows, or requests *
-        width if that is less).  max_context bounds the requests' lengths and only plans the launches."""
+        width if that is less).  max_context bounds the requests' lengths and only plans the launches.  A
+        token outside the vocabulary makes its request's logits NaN from then on."""
         c, cache = self.weights.config, self.cache
         device = cache.pool.device
         if not isinstance(tokens, torch.Tensor):
             if len(tokens) != cache.requests:
                 raise ValueError(f"one list of tokens for each of {cache.requests} requests")
+            if not isinstance(counts, torch.Tensor) and any(n > len(t) for n, t in zip(counts, tokens)):
+                raise ValueError("a count is more than its request's tokens")
             width = max(1, max(len(t) for t in tokens))
             tokens = torch.tensor([list(t) + [0] * (width - len(t)) for t in tokens], dtype=torch.int32).to(device)
         if tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != cache.requests or tokens.shape[1] < 1:
             raise ValueError(f"tokens must be int32 ({cache.requests}, width)")
+        if tokens.device != device:
+            raise ValueError(f"the tokens are on {tokens.device}, the cache on {device}")
         if not isinstance(counts, torch.Tensor):
             if len(counts) != cache.requests or min(counts) < 0 or max(counts) > tokens.shape[1]:
                 raise ValueError(f"{cache.requests} counts of 0 to {tokens.shape[1]} tokens, got {counts}")

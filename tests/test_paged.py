@@ -201,8 +201,10 @@ def test_paged_cache_and_decoder_refuse_before_they_reach_the_gpu():
             cache.reserve([1, 1], rows)
     with pytest.raises(ValueError):  # tensors on the host
         cache.reserve([1, 1])
-    with pytest.raises(ValueError):
-        cache.fork(0, [1])
+    for call in (lambda: cache.fork(0, [1]), lambda: cache.fork(2, [1]), lambda: cache.fork(0, [2]),
+                 lambda: cache.fork(0, [-1]), lambda: cache.release([2]), lambda: cache.release([-1])):
+        with pytest.raises(ValueError):
+            call()
     weights = random_weights(cfg, "cpu")
     with pytest.raises(ValueError):
         PagedDecoder(weights, PagedCache(DecoderConfig(), 1, 16, 1, 1, "cpu"))

@@ -304,6 +304,10 @@ def test_requests_that_do_not_fit_are_left_as_they_were():
     with pytest.raises(ValueError):
         model.extend([[1], [], []], [2, 0, 0])
     with pytest.raises(ValueError):
+        model.extend([[1], [1, 2], []], [2, 2, 0])  # within the width, but more than request 0's tokens
+    with pytest.raises(ValueError):
+        model.extend(torch.zeros((3, 1), dtype=torch.int32), [1, 1, 1])  # on the host
+    with pytest.raises(ValueError):
         model.extend([[1] * 65, [], []], [65, 0, 0])
     with pytest.raises(ValueError):
         model.extend(torch.zeros((2, 1), dtype=torch.int32, device="cuda"), [1, 1])
