@@ -41,10 +41,10 @@ __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo 
 // Requests are taken or refused between the two by the sums of what was asked for.
 //
 // Bound by its chain of loads and barriers, and in a large cache by the references, which one CU reads
-// at about 150 GB/s (512 KB for 131072 pages).  One column and four references a thread at a time are best for
-// a step's few columns (eight beams 5.6 us, 9.6 with eight and 16), those for many prompts' (a round of 764
-// requests 50, 104 with
-// the others).
+// at about 150 GB/s (512 KB for 131072 pages).  One column and four references a thread at a time are best
+// for a step's few columns (eight beams 5.6 us, 9.6 with eight and 16), four and 16 for many prompts' (a
+// round of 764 requests 46; 50 with eight and 16, 104 with one and four).  Columns in turn among a wavefront's
+// lanes, for neighbouring accesses, took 150: a lane's next column is then many requests on.
 constexpr int kReserveThreads = 1024, kReserveWaves = kReserveThreads / 64;
 constexpr int kMaxRequests = IMQ_PAGED_MAX_REQUESTS;
 
@@ -1728,7 +1728,7 @@ int32_t imq_paged_reserve(const imq_paged_cache* cache, const int32_t* counts, c
                 chunk->copies, cache->requests, cache->columns, cache->pages, shift, chunk->rows};
   // at most this many columns: those that the rows fill, and two part-full ones for each request
   const int64_t most = chunk->rows / cache->page_size + 2 * (int64_t)cache->requests;
-  const auto kernel = most <= 2 * kReserveThreads ? reserve_kernel<1, 4, 4096> : reserve_kernel<8, 16, 24576>;
+  const auto kernel = most <= 2 * kReserveThreads ? reserve_kernel<1, 4, 4096> : reserve_kernel<4, 16, 24576>;
   hipLaunchKernelGGL(kernel, dim3(1), dim3(kReserveThreads), 0, st, a);
   code = launched("reserve");
   if (code != IMQ_OK) return code;
