@@ -415,3 +415,60 @@ def test_every_row_in_the_same_place_gives_the_same_bits(env):
     first = b.run(n_).clone()
     for _ in range(3):
         assert torch.equal(b.run(n_), first)
+
+
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,extra", [(9, 32, 8, 128, 0), (300, 16, 8, 256, 64)])
+def test_a_write_over_its_own_queries(env, rows, heads, kv_heads, dim, extra):
+    torch, n_ = env
+    announce("paged write in place", rows, heads, dim)
+    gen = _gen(torch, rows)
+    q, k, v = (_wide(torch, rows, h, dim, extra, gen) for h in (heads, kv_heads, kv_heads))
+    weight = torch.ones(dim, device="cuda", dtype=torch.bfloat16)
+    positions = torch.arange(rows, dtype=torch.int32, device="cuda")
+    slots = positions.clone()
+    slots[2] = -1
+    apart, over = q.clone(), q
+    pools = [torch.zeros((rows // 16 + 1, kv_heads, 16, dim), device="cuda", dtype=torch.bfloat16) for _ in range(4)]
+    n_.paged_write(q.clone(), k, v, weight, weight, positions, slots, apart, *pools[:2], theta=1e4, eps=1e-6)
+    n_.paged_write(over, k, v, weight, weight, positions, slots, over, *pools[2:], theta=1e4, eps=1e-6)
+    assert torch.equal(over, apart)
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
+
+
+@pytest.mark.parametrize("dim,page", [(128, 512), (256, 256)])
+def test_pages_past_four_gigabytes(env, dim, page):
+    """A cache whose last pages lie past 2^32 bytes (and 2^31 values): written, attended over by both kinds of
+    launches and copied as the same pages of a small one are."""
+    torch, n_ = env
+    announce("paged cache past 32 bits", dim)
+    pages, kv_heads, heads = 4400, 8, 16
+    gen = _gen(torch, dim)
+    far = torch.empty((2, pages, kv_heads, page, dim), device="cuda", dtype=torch.bfloat16)  # 9.2 GB, mostly never touched
+    near = torch.randn((2, 5, kv_heads, page, dim), device="cuda", generator=gen).to(torch.bfloat16)
+    far[:, -5:] = near
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    tables = ints([0, 3, 1], [4, 2, -1])
+    tables_far = torch.where(tables >= 0, tables + pages - 5, tables)
+    weight = torch.ones(dim, device="cuda", dtype=torch.bfloat16)
+    for counts, ends in (((1, 1), (3 * page - 7, page + 9)), ((200, 1), (2 * page + 90, 2 * page))):
+        rows = sum(counts)
+        q, k, v = (torch.randn((rows, h, dim), device="cuda", generator=gen).to(torch.bfloat16) for h in (heads, kv_heads, kv_heads))
+        positions = torch.cat([torch.arange(e - c, e) for c, e in zip(counts, ends)]).int().cuda()
+        owner = torch.cat([torch.full((c,), r) for r, c in enumerate(counts)]).cuda()
+        starts, outs = ints(0, counts[0], rows), []
+        for pool, table in ((near, tables), (far, tables_far)):
+            slots = table[owner, (positions // page).long()] * page + positions % page
+            turned, out = torch.empty_like(q), torch.empty_like(q)
+            n_.paged_write(q, k, v, weight, weight, positions, slots, turned, pool[0], pool[1], theta=1e6, eps=1e-6)
+            n_.paged_attention(turned, pool[0], pool[1], table, starts, ints(*ends), out, dim ** -0.5)
+            outs.append(out)
+        assert outs[0].isfinite().all() and torch.equal(*outs)
+        assert torch.equal(far[:, -5:], near)
+    # a shared page, part-filled: its new owner gets the last page, copied in both planes
+    refs = torch.ones(pages, dtype=torch.int32, device="cuda")
+    refs[pages - 3], refs[pages - 1] = 2, 0
+    chunk = [ints(0, 0, 0), ints(0, 0), ints(0, 0), ints(0), ints(0), torch.zeros((2, 2), dtype=torch.int32, device="cuda")]
+    n_.paged_reserve(ints([pages - 3], [pages - 3]), ints(10, 10), refs, ints(1, 0), page, *chunk, pool=far)
+    assert chunk[2].tolist() == [0, 0] and chunk[5].tolist() == [[pages - 3, pages - 1], [-1, -1]]
+    assert chunk[4].tolist() == [(pages - 1) * page + 10]
+    assert torch.equal(far[:, -1], near[:, 2]) and torch.equal(far[:, -5:-1], near[:, :4])
