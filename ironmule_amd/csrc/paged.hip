@@ -674,7 +674,7 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {  // v_pk_
 // swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
 // over the softmax and P V, and no barrier before the wavefronts' results are joined.
-// Bound by memory: 32 requests of up to 8000 tokens, 32 heads on 8 of 128 (669 MB), 118 us, 5.7 TB/s, and 6 us
+// Bound by memory: 32 requests of up to 8000 tokens, 32 heads on 8 of 128 (669 MB), in 109 us, 6.1 TB/s, and 6 us
 // for the second launch.  One of 777 tokens 7.4 and 4.8 us: the chain of starts, lengths, table and keys, each
 // a load after the last.  Parts of four blocks: a request of 8000 tokens 17 us instead of 14.
 constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 8;
@@ -698,7 +698,13 @@ __device__ __forceinline__ lds_char part_of(int w, uint32_t at0, uint32_t at1, u
   return (lds_char)(uintptr_t)(w & 2 ? (w & 1 ? at3 : at2) : w & 1 ? at1 : at0);
 }
 
-template <int D>
+template <bool ONCE>
+__device__ __forceinline__ u32x4_t load_piece(const char* at) {
+  const u32x4_t* const p = reinterpret_cast<const u32x4_t*>(at);
+  return ONCE ? __builtin_nontemporal_load(p) : *p;
+}
+
+template <int D, bool ONCE>
 __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const Request& s, int request, int place, int from,
                                             int to, int slot, char* l0, char* l1, char* l2, char* l3, float (*tops)[16],
                                             float (*sums)[16]) {
@@ -756,7 +762,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
       for (int b = 0; b < 2; ++b) {
         const char* const base = reinterpret_cast<const char*>(a.k_pages) + group_offset(b ? page1 : page0, block, b);
 #pragma unroll
-        for (int t = 0; t < T; ++t) kr[b][t] = *reinterpret_cast<const u32x4_t*>(base + k_lane + 64 * t);
+        for (int t = 0; t < T; ++t) kr[b][t] = load_piece<ONCE>(base + k_lane + 64 * t);
       }
     };
     auto load_v = [&](int page0, int page1, int block) {
@@ -765,7 +771,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
         const char* const base = reinterpret_cast<const char*>(a.v_pages) + group_offset(b ? page1 : page0, block, b);
 #pragma unroll
         for (int i = 0; i < V / 2; ++i)
-          vr[b * (V / 2) + i] = *reinterpret_cast<const u32x4_t*>(base + v_lane + 1024 * i);
+          vr[b * (V / 2) + i] = load_piece<ONCE>(base + v_lane + 1024 * i);
       }
     };
     int now0 = page_of(at, 0), now1 = page_of(at, 1);
@@ -906,7 +912,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
 }
 
 // Workgroup `index` of a launch over tiles of few queries.
-template <int D>
+template <int D, bool ONCE>
 __device__ __forceinline__ void rows_workgroup(const AttendArgs& a, int index, char* l0, char* l1, char* l2, char* l3,
                                                float (*tops)[16], float (*sums)[16]) {
   const int unit = index / a.Hkv, head = index % a.Hkv;
@@ -925,8 +931,8 @@ __device__ __forceinline__ void rows_workgroup(const AttendArgs& a, int index, c
     // a tile not whole here: the workgroup's first partial result, or its last
     const int slot = length == q.blocks ? -1 : 2 * unit + (x != x0);
     if (x != x0) __syncthreads();
-    attend_rows<D>(a, head, q, request, place, q.block0 + (in << a.grain), q.block0 + ((in + length) << a.grain), slot, l0, l1, l2, l3,
-                   tops, sums);
+    attend_rows<D, ONCE>(a, head, q, request, place, q.block0 + (in << a.grain), q.block0 + ((in + length) << a.grain), slot,
+                         l0, l1, l2, l3, tops, sums);
     x += length;
   }
 }
@@ -1533,20 +1539,21 @@ __device__ __forceinline__ void merge_tile(const AttendArgs& a, int index, Merge
 // last of them.  A mixed batch of 24 requests in 87 us, 93 in turns of 32 and 102 the other way round.  (In turns
 // of eight, one workgroup of each kind per XCD, half of an XCD's shader engines got all of the tiles: 144
 // against 117 in turns of 32.)
-enum { kFew = 1, kMany = 2 };
+enum { kFew = 1, kMany = 2, kFewOnce = 4 };  // (kFewOnce: kFew, whose keys and values one workgroup reads)
 
 template <int D, int KINDS>
 __global__ __launch_bounds__(kThreads, D == 128 ? 2 : 1) void attend_kernel(AttendArgs few, AttendArgs many, int many_groups) {
   __shared__ __attribute__((aligned(16))) char lds0[kArray], lds1[kArray];
   __shared__ float tops[4][16], sums[4][16];
-  if (KINDS == kFew && D == 128) {
-    rows_workgroup<D>(few, blockIdx.x, lds0, lds1, nullptr, nullptr, tops, sums);
+  constexpr bool ONCE = KINDS == kFewOnce, FEW = KINDS == kFew || ONCE;
+  if (FEW && D == 128) {
+    rows_workgroup<D, ONCE>(few, blockIdx.x, lds0, lds1, nullptr, nullptr, tops, sums);
   } else {
     __shared__ __attribute__((aligned(16))) char lds2[kArray], lds3[kArray];
-    const bool is_few = KINDS == kFew || (KINDS == (kFew | kMany) && (int)blockIdx.x >= many_groups);
+    const bool is_few = FEW || (KINDS == (kFew | kMany) && (int)blockIdx.x >= many_groups);
     const int index = KINDS == (kFew | kMany) && is_few ? blockIdx.x - many_groups : blockIdx.x;
-    if ((KINDS & kFew) && is_few)
-      rows_workgroup<D>(few, index, lds0, lds1, lds2, lds3, tops, sums);
+    if (KINDS != kMany && is_few)
+      rows_workgroup<D, ONCE>(few, index, lds0, lds1, lds2, lds3, tops, sums);
     else if (KINDS & kMany)
       tile_workgroup<D>(many, index, lds0, lds1, lds2, lds3);
   }
@@ -1617,7 +1624,14 @@ struct AttendLaunch {
 
 struct AttendPlan {
   AttendLaunch few, many;
+  bool once;  // one row for each request: its keys and values are read by one workgroup per KV head
 };
+
+// Of more keys and values than the last-level cache holds (256 MB), which are read once, nothing is kept in the
+// caches: 32 steps over up to 8000 tokens (669 MB) in 115 us, 125 with plain loads.  Fewer stay there for
+// the next call (32768 tokens, 134 MB: 31 us, and 33), and two tiles of a request share them (8 tokens each
+// of four requests: 27 us, and 32).
+constexpr int64_t kCached = 256ll << 20;
 
 // Requests of up to kRowsMost queries go to rows_workgroup, longer ones to tile_workgroup.  The
 // host knows the sums only: where the average request stays within kRowsMost the first serves all.
@@ -1632,6 +1646,7 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
   const int resident = head_dim == 128 ? kWorkgroups<128> : kWorkgroups<256>;
   // (a window's keys before the rows' own, and the parts of blocks at both ends)
   const int64_t keys = window ? std::min(max_context, (int64_t)window + rows) : max_context;
+  p.once = all_few && rows <= requests && Hq / Hkv <= kRowsTile && with * keys * Hkv * head_dim * 4 > kCached;
   if (all_few || some_few) {
     AttendLaunch& l = p.few;
     l.width = kRowsTile;
@@ -1692,7 +1707,7 @@ void launch_attend(const AttendPlan& p, char* space, const AttendArgs& args, hip
   const AttendArgs few = with_launch(args, p.few, D, space);
   const AttendArgs many = with_launch(args, p.many, D, space + attend_space(p.few, args.Hkv, D));
   const int few_groups = (int)p.few.workgroups * args.Hkv, many_groups = (int)p.many.workgroups * args.Hkv;
-  const auto kernel = !p.many.width  ? attend_kernel<D, kFew>
+  const auto kernel = !p.many.width  ? p.once ? attend_kernel<D, kFewOnce> : attend_kernel<D, kFew>
                       : !p.few.width ? attend_kernel<D, kMany>
                                      : attend_kernel<D, (kFew | kMany)>;
   hipLaunchKernelGGL(kernel, dim3(few_groups + many_groups), dim3(kThreads), 0, stream, few, many, many_groups);
