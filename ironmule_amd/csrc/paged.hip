@@ -419,7 +419,8 @@ __global__ __launch_bounds__(kMaxRequests) void reorder_lengths_kernel(int32_t* 
 // bytes.  The first heads' loads are in flight while the row's angles are computed (in double: positions
 // are large, and the angle is the product).  Two roundings to bf16, as imq_qk_norm_rope: the norm's result
 // (what the model's norm gives) and the turned value.
-// Bound by memory: 4099 rows of 32 heads of 256 (134 MB read and written) in 22.5 us, 6.0 TB/s; single
+// Bound by memory: 4099 rows of 32 heads of 256 (134 MB read and written) in 22.5 us where they are in the
+// last-level cache, in 28 with new ones; single
 // 2-byte values a lane took 34.  The slot is looked at after the loads: before them, 32.  256 to 512
 // threads are alike there, 320 and more best for a few rows (five rows 3.8 us, 4.2 with 256); a number of
 // threads by the row's heads 26.
@@ -669,7 +670,8 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {  // v_pk_
 // blocks is cut into `units` equal parts whatever tiles they belong to, a workgroup takes one, tile
 // after tile, and each of its four wavefronts a quarter of a tile's keys there, 32 at a time.
 // Scores are K Q^T on v_mfma_f32_16x16x32_bf16, so that a lane holds keys of one query: P^T is then
-// the B operand of V^T P^T without leaving its lane (keys 4 g .. of two 16-key tiles).  K goes from
+// the B operand of V^T P^T without leaving its lane (keys 4 g .. of two 16-key tiles), rounded to bf16
+// (a relative 2^-8 at most; the maxima, the sums and P V itself stay in fp32).  K goes from
 // its page to the A operand directly; V goes through the wavefront's own LDS by rows, 32-byte pieces
 // swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
