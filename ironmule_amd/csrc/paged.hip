@@ -643,6 +643,10 @@ struct BlocksOf {
   __device__ __forceinline__ int operator()(const Request& q) const { return q.blocks; }
 };
 
+struct One {
+  __device__ __forceinline__ int operator()(const Request&) const { return 1; }
+};
+
 __device__ __forceinline__ int ceil_of(int a, int b) { return (a + b - 1) / b; }
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
@@ -919,6 +923,15 @@ __device__ __forceinline__ void rows_workgroup(const AttendArgs& a, int index, c
                                                float (*tops)[16], float (*sums)[16]) {
   const int unit = index / a.Hkv, head = index % a.Hkv;
   Lanes<kRowsTile, kRowsBlock> lanes(a);
+  if (a.units == 0) {  // whole tiles (rows_alone)
+    Line<Lanes<kRowsTile, kRowsBlock>, One> tiles(lanes, One());
+    Request q;
+    int request, start;
+    if (!tiles.find(unit, &q, &request, &start) || unit < start || unit - start >= q.tiles) return;
+    attend_rows<D, ONCE>(a, head, q, request, unit - start, q.block0, q.block0 + (q.blocks << a.grain), -1, l0, l1, l2, l3, tops,
+                         sums);
+    return;
+  }
   Line<Lanes<kRowsTile, kRowsBlock>, BlocksOf> line(lanes, BlocksOf());
   const int part = part_length(a, line.total, kRowsLeast);
   if ((int64_t)unit * part >= line.total) return;
@@ -1635,6 +1648,12 @@ struct AttendPlan {
 // of four requests: 27 us, and 32).
 constexpr int64_t kCached = 256ll << 20;
 
+// The keys (of heads of 128) up to which tiles of few queries are left whole, one workgroup each and no second launch,
+// rather than cut into equal parts of all their blocks.  One request: 512 keys 9.3 us and 11.3 cut, 777 equal, 1024
+// 13.7 and 11.9; eight requests (64 workgroups): 512 keys 9.5 and 15.3, 1024 13.8 and 16.5, 2000 22.8
+// and 22.1; 32 requests: 1024 17.8 and 23.8, 2000 29 and 33, 4000 68 and 62.
+int64_t rows_alone(int64_t workgroups) { return workgroups >= 128 ? 2048 : workgroups >= 32 ? 1024 : 768; }
+
 // Requests of up to kRowsMost queries go to rows_workgroup, longer ones to tile_workgroup.  The
 // host knows the sums only: where the average request stays within kRowsMost the first serves all.
 // A workgroup with nothing to do costs its launch all the same (1000 of them 10 us): no more are launched than
@@ -1657,7 +1676,8 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
     const int64_t line = l.tiles * (keys / kRowsBlock + 2);
     l.units = std::min<int64_t>(ceil_div(resident, Hkv),
                                 ceil_div(line, kRowsLeast));
-    l.workgroups = l.units;
+    if (keys * head_dim <= rows_alone(l.tiles * Hkv) * 128) l.units = 0;
+    l.workgroups = l.units ? l.units : l.tiles;
     l.slots = l.units > 1 ? 2 * l.units : 0;  // a part's first tile and its last
   }
   if (!all_few) {

@@ -249,13 +249,14 @@ def test_write_agrees_with_the_decode_kernel(env):
 # ------------------------------------------------------------------ attention
 
 class _Batch:
-    def __init__(self, torch, requests, heads, kv_heads, dim, page, seed, extra=0, spare=7):
-        """`requests`: (new tokens, tokens with them) each; pages scattered, what lies past a request's end NaN."""
+    def __init__(self, torch, requests, heads, kv_heads, dim, page, seed, extra=0, spare=7, room=0):
+        """`requests`: (new tokens, tokens with them) each; pages scattered, what lies past a request's end NaN;
+        tables for `room` tokens at least (where little room is left tiles stay whole)."""
         gen = _gen(torch, seed)
         needs = [-(-end // page) for _, end in requests]
         pages = sum(needs) + spare
         order = torch.randperm(pages, device="cuda", generator=gen).to(torch.int32)
-        self.tables = torch.full((len(requests), max(needs) + 1), -1, dtype=torch.int32, device="cuda")
+        self.tables = torch.full((len(requests), max(max(needs) + 1, room // page)), -1, dtype=torch.int32, device="cuda")
         at = 0
         for r, need in enumerate(needs):
             self.tables[r, :need] = order[at:at + need]
@@ -310,6 +311,25 @@ def test_attention_against_64_bits(env, heads, kv_heads, dim, batch, page):
     torch, n_ = env
     announce("paged attention", heads, kv_heads, dim, BATCHES[batch], page)
     _Batch(torch, BATCHES[batch], heads, kv_heads, dim, page, seed=batch).check(torch, n_)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", HEADS)
+@pytest.mark.parametrize("batch", range(len(BATCHES)))
+def test_attention_with_room_in_the_tables_against_64_bits(env, heads, kv_heads, dim, batch):
+    torch, n_ = env
+    announce("paged attention, room", heads, kv_heads, dim, BATCHES[batch])
+    _Batch(torch, BATCHES[batch], heads, kv_heads, dim, 32, seed=batch + 20, room=9000).check(torch, n_)
+
+
+@pytest.mark.parametrize("requests,heads,kv_heads,dim", [
+    ([(1, 760)], 32, 8, 128), ([(1, 1000)], 32, 8, 128), ([(1, 380)], 16, 8, 256), ([(1, 500)], 16, 8, 256),
+    ([(1, 1000 - i) for i in range(4)], 32, 8, 128), ([(1, 2000 - 90 * i) for i in range(16)], 32, 8, 128),
+    ([(1, 2040)] * 15, 32, 8, 128), ([(2, 1000 + i) for i in range(20)], 64, 8, 256), ([(4, 1500)] * 70, 16, 2, 128)])
+def test_steps_around_the_lengths_that_leave_tiles_whole(env, requests, heads, kv_heads, dim):
+    torch, n_ = env
+    announce("paged attention, whole or cut", len(requests), requests[0], heads, dim)
+    for room in (0, 8192):
+        _Batch(torch, requests, heads, kv_heads, dim, 16, seed=11, room=room).check(torch, n_)
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim", HEADS[:3])
@@ -372,8 +392,8 @@ def test_infinities_and_nans_stay_where_they_are_seen(env, dim, requests):
     the dimensions concerned), every other row is as if they were not there; at the edges of windows too."""
     torch, n_ = env
     announce("paged attention, not finite", dim, requests)
-    for window in (0, 50):
-        b = _Batch(torch, requests, 8, 2, dim, 16, seed=dim + window)
+    for window, room in ((0, 0), (50, 0), (0, 9000), (50, 9000)):
+        b = _Batch(torch, requests, 8, 2, dim, 16, seed=dim + window, room=room)
         inf, nan = float("inf"), float("nan")
         for pool, position, at, value in ((b.v, 195, 3, inf), (b.v, 160, 7, nan), (b.v, 100, slice(None), -inf),
                                           (b.v, 199, 0, nan), (b.k, 170, 5, nan)):
@@ -384,12 +404,13 @@ def test_infinities_and_nans_stay_where_they_are_seen(env, dim, requests):
         assert not got[int(b.starts[0]):int(b.starts[1])].isfinite().all() and got[-1, 0].isfinite().all()
 
 
-def test_bad_table_entries_and_odd_requests(env):
+@pytest.mark.parametrize("room", [0, 9000])
+def test_bad_table_entries_and_odd_requests(env, room):
     """Pages outside the pool are left out, a request that ends before its rows begin sees nothing, ends past the tables
     and rows past the batch are cut off; nothing outside is read (the host refuses the rest)."""
     torch, n_ = env
     announce("paged attention, bad tables")
-    b = _Batch(torch, [(1, 100), (20, 120), (1, 40), (3, 3)], 8, 2, 128, 16, seed=2)
+    b = _Batch(torch, [(1, 100), (20, 120), (1, 40), (3, 3)], 8, 2, 128, 16, seed=2, room=room)
     pages = b.k.shape[0]
     b.tables[0, 2], b.tables[1, 0], b.tables[1, 7], b.tables[2, :3] = -1, pages, 2**31 - 1, -5
     b.check(torch, n_)
