@@ -118,8 +118,9 @@ IMQ_API int32_t imq_paged_attention(const uint16_t* q, int64_t ldq, const uint16
 
 /* The `count` best continuations of each group of `beams` beams (rows group * beams ..):
  *   key(b, v) = scores[b] + logits[b][v] - log(sum_u exp(logits[b][u]))      over all b, v of a group
- * compared in double, ties to the lowest (b, v).  logits: fp32 or bf16 rows of `vocab` values, ld
- * apart.  `finished` (may be null): a beam with a non-zero flag offers only itself, token eos with
+ * compared in double (inside a beam: the logits themselves), ties to the lowest (b, v).  The log sum is good
+ * to a few units of 2^-24 whatever the size of the logits, which may be masked with the lowest finite
+ * value of their type as well as with -inf.  logits: fp32 or bf16 rows of `vocab` values, ld apart.  `finished` (may be null): a beam with a non-zero flag offers only itself, token eos with
  * its score.  Values that are NaN or -inf, and beams whose score or sum is not finite, offer nothing.
  * Outputs (groups, count), the best first: the key as fp32, the parent row (over all groups), the
  * token, and whether the continuation is finished (its parent was, or the token is eos); where there

@@ -224,11 +224,14 @@ __global__ __launch_bounds__(kThreads) void select_slice_kernel(const void* __re
     const float higher = fmaxf(most, wave_max(mine)), base = higher == -INFINITY ? 0.0f : higher;
     if (block) sum *= (double)__builtin_amdgcn_exp2f((most - base) * kLog2e);
     most = higher;
+    // Eight at a time in fp32 (a NaN stays one).  The difference first: base * log2(e) as a number of its own is
+    // rounded to its own size, which every term would carry, and is infinite for a base of the lowest finite
+    // value; the difference is as good as its own size, and the largest value's term is 1.
 #pragma unroll
-    for (int e = 0; e < E; e += 8) {  // eight at a time in fp32 (a NaN stays one)
+    for (int e = 0; e < E; e += 8) {
       float part = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) part += __builtin_amdgcn_exp2f(fmaf(x[e + k], kLog2e, -base * kLog2e));
+      for (int k = 0; k < 8; ++k) part += __builtin_amdgcn_exp2f((x[e + k] - base) * kLog2e);
       sum += (double)part;
     }
     have = wave_best<E>(x, mine, [&](int e) { return v0 + 64 * N * (e / N) + e % N; }, count, have, best[wave], some[wave]);
@@ -276,10 +279,12 @@ struct SelectArgs {
 };
 
 // A workgroup per group.  A wavefront per beam at a time: the beam's log sum, and the best of its slices'
-// candidates in order; then a thread per (beam, entry) counts the better ones of the other beams.
+// candidates in order; then a thread per (beam, entry) counts the better ones of the other beams.  A key is
+// (value - largest) + (score - log sum of exp(value - largest)): the largest value alone may be of any size.
 __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(Slices s, SelectArgs a) {
   constexpr int kE = 8;
   __shared__ double shift[kMaxBeams];  // score - log sum, of a finished beam the score
+  __shared__ float tops[kMaxBeams];    // the largest value, of a finished beam 0
   __shared__ int counts[kMaxBeams];
   __shared__ uint64_t best[kMaxBeams][kMaxCount];
   __shared__ uint64_t some[kMergeThreads / 64][kSome + kRankStep];
@@ -289,7 +294,7 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(Slices s, S
     const float score = a.scores[row];
     int have = 0;
     if (a.finished && a.finished[row]) {
-      if (lane == 0) shift[b] = (double)score, best[b][0] = rank_of(0.0f, a.eos);
+      if (lane == 0) shift[b] = (double)score, tops[b] = 0.0f, best[b][0] = rank_of(0.0f, a.eos);
       have = isfinite(score) ? 1 : 0;
     } else {
       const int64_t at = (int64_t)row * s.slices;
@@ -303,9 +308,9 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(Slices s, S
         sum += m == -INFINITY && z == 0.0 ? 0.0 : z * exp((double)m - (most == -INFINITY ? 0.0f : most));
       }
       sum = wave_total(sum);
-      const double v = (double)score - ((double)most + log(sum));
-      if (lane == 0) shift[b] = v;
-      if (isfinite(v)) {  // (a score, a value or a sum that is not finite: nothing is offered)
+      const double v = (double)score - log(sum);
+      if (lane == 0) shift[b] = v, tops[b] = most;
+      if (isfinite(v) && isfinite(most)) {  // (a score, a value or a sum that is not finite: nothing is offered)
         const int all = s.slices * a.count;
         for (int i0 = 0; i0 < all; i0 += 64 * kE) {
           float x[kE], mine = -INFINITY;
@@ -327,7 +332,7 @@ __global__ __launch_bounds__(kMergeThreads) void select_merge_kernel(Slices s, S
   __syncthreads();
   int all = 0;
   for (int b = 0; b < a.beams; ++b) all += counts[b];
-  auto key_of = [&](int b, int i) { return shift[b] + (double)value_of((uint32_t)(best[b][i] >> 32)); };
+  auto key_of = [&](int b, int i) { return ((double)value_of((uint32_t)(best[b][i] >> 32)) - (double)tops[b]) + shift[b]; };
   for (int item = threadIdx.x; item < a.beams * a.count; item += kMergeThreads) {
     const int b = item / a.count, i = item % a.count;
     if (i >= counts[b]) continue;
