@@ -423,6 +423,10 @@ def qmv_workspace_bytes(shapes) -> int:
 def _grouped_launch(probs, count: int, m: int, dtype: torch.dtype, device, stream, workspace=None) -> None:
     """imq_qmv_grouped, through imq_qmv_grouped_ws with this stream's workspace (or the given one) when the
     library wants one (M >= 3 and few rows: the groups are split over more workgroups)."""
+    if workspace is not None and not (workspace.dtype is torch.float32 and workspace.is_contiguous()
+                                      and workspace.device == device):
+        raise ValueError(f"the workspace must be a contiguous fp32 tensor on {device}, got {workspace.dtype} on "
+                         f"{workspace.device}")
     nbytes = int(lib().imq_qmv_grouped_workspace(probs, count, m)) if m >= 3 else 0
     if nbytes == 0:
         _check(lib().imq_qmv_grouped(probs, count, m, GROUP_SIZE, BITS, _DTYPE_CODE[dtype],
@@ -460,9 +464,9 @@ def qmv_grouped(weights: list[tuple[torch.Tensor, torch.Tensor, torch.Tensor]],
                 out_dtype: torch.dtype = torch.bfloat16, stream=None,
                 workspace: torch.Tensor | None = None) -> list[torch.Tensor]:
     """One launch for up to 8 weights, each with its own (M, K_i) activation rows (the
-    same tensor may serve several weights, e.g. q/k/v); returns the (M, N_i) outputs.  `workspace`: fp32,
-    zero before its first use, in place of the stream's own (qmv_workspace_bytes; calls that share one
-    must not overlap)."""
+    same tensor may serve several weights, e.g. q/k/v); returns the (M, N_i) outputs.  `workspace`: whole fp32
+    on the weights' device, zero before its first use, in place of the stream's own (qmv_workspace_bytes;
+    calls that share one must not overlap; one that is too small is used as far as it goes)."""
     count = len(weights)
     if not 1 <= count <= MAX_PROBLEMS or len(xs) != count:
         raise ValueError(f"1 to {MAX_PROBLEMS} weights with one activation each")
