@@ -70,7 +70,10 @@ class PagedCache:
         rows = self.rows if rows is None else rows
         if not 1 <= rows <= self.rows:
             raise ValueError(f"a step of this cache has 1 to {self.rows} rows, got {rows}")
-        self.counts.copy_(torch.as_tensor(counts, dtype=torch.int32))
+        counts = torch.as_tensor(counts, dtype=torch.int32)
+        if counts.shape != (self.requests,):
+            raise ValueError(f"one count for each of {self.requests} requests, got counts of shape {tuple(counts.shape)}")
+        self.counts.copy_(counts)
         _native.paged_reserve(self.tables, self.lengths, self.refs, self.counts, self.page_size, self.starts,
                               self.ends, self.status, self.positions[:rows], self.slots[:rows], self.copies,
                               pool=self.pool)
