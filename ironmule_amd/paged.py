@@ -163,16 +163,18 @@ class PagedDecoder:
 
         tokens: lists of numbers per request, or an int32 tensor (requests, width) on the GPU with counts
         there too; then `rows` bounds the sum of the counts (default: the cache's rows, or requests *
-        width if that is less).  max_context bounds the requests' lengths and only plans the launches.  A
-        token outside the vocabulary makes its request's logits NaN from then on."""
+        width if that is less), and a request with a count past its tokens is refused (status 2).  max_context
+        bounds the requests' lengths and only plans the launches.  A token outside the vocabulary makes its
+        request's logits NaN from then on."""
         c, cache = self.weights.config, self.cache
-        device = cache.pool.device
+        device, limits = cache.pool.device, None
         if not isinstance(tokens, torch.Tensor):
             if len(tokens) != cache.requests:
                 raise ValueError(f"one list of tokens for each of {cache.requests} requests")
             if not isinstance(counts, torch.Tensor) and any(n > len(t) for n, t in zip(counts, tokens)):
                 raise ValueError("a count is more than its request's tokens")
-            width = max(1, max(len(t) for t in tokens))
+            limits = [len(t) for t in tokens]
+            width = max(1, *limits)
             tokens = torch.tensor([list(t) + [0] * (width - len(t)) for t in tokens], dtype=torch.int32).to(device)
         if tokens.dtype != torch.int32 or tokens.dim() != 2 or tokens.shape[0] != cache.requests or tokens.shape[1] < 1:
             raise ValueError(f"tokens must be int32 ({cache.requests}, width)")
@@ -185,6 +187,9 @@ class PagedDecoder:
             if total > cache.rows:
                 raise ValueError(f"a step of this cache has at most {cache.rows} rows, got {total}")
             rows = max(1, total) if rows is None else rows
+        else:  # (-1: malformed, which the reservation refuses)
+            limit = tokens.shape[1] if limits is None else torch.tensor(limits, dtype=torch.int32).to(counts.device)
+            counts = counts.masked_fill(counts > limit, -1)
         if rows is None:
             rows = min(cache.rows, cache.requests * tokens.shape[1])
         cache.reserve(counts, rows)
