@@ -251,7 +251,8 @@ class PagedDecoder:
     def prefill(self, prompts) -> torch.Tensor:
         """Appends prompts[r] (a list of tokens, may be empty) to every request r, in chunks of at most the
         cache's rows; returns the logits (requests, vocab) of the last token of each (NaN where it is
-        empty).  Raises RuntimeError if the cache has not the pages (requests then hold a part)."""
+        empty).  Raises RuntimeError if the cache has not the pages: a request then holds the chunks of its prompt
+        up to the first that did not fit, as many tokens more as its length says."""
         cache = self.cache
         if len(prompts) != cache.requests:
             raise ValueError(f"one prompt for each of {cache.requests} requests")
@@ -263,14 +264,15 @@ class PagedDecoder:
             for a, p in zip(at, prompts):
                 counts.append(min(room, len(p) - a))
                 room -= counts[-1]
-            chunk = self.extend([p[a:a + n] for a, p, n in zip(at, prompts, counts)], counts)
+            chunks = [p[a:a + n] for a, p, n in zip(at, prompts, counts)]
+            if logits is None:
+                logits = self.extend(chunks, counts)
+            else:  # (nothing more of a request that was refused a chunk)
+                new = torch.tensor(counts, dtype=torch.int32).to(logits.device)
+                chunk = self.extend(chunks, torch.where(refused == 0, new, 0), rows=max(1, sum(counts)))
+                logits = torch.where((new > 0)[:, None], chunk, logits)
             refused |= cache.status
             at = [a + n for a, n in zip(at, counts)]
-            if logits is None:
-                logits = chunk
-            else:
-                new = torch.tensor(counts, device=chunk.device) > 0
-                logits = torch.where(new[:, None], chunk, logits)
         if bool(refused.any()):
             raise RuntimeError("the cache has too few pages, or a request too few columns, for these prompts")
         return logits

@@ -53,3 +53,29 @@ def test_a_count_past_the_tokens_refuses_its_request():
         torch.cuda.synchronize()
         assert models[2].cache.lengths.tolist() == models[1].cache.lengths.tolist()
         assert models[2].cache.status.tolist() == [[0, 2, 0], [0, 0, 0], [2, 0, 0]][step]
+
+
+def test_a_refused_prompt_leaves_what_it_begins_with():
+    """A chunk that does not fit ends its request's prompt, though the last and smaller one would fit; the other
+    prompts go on, and the rest can be taken later where pages have become free."""
+    import torch
+
+    from ironmule_amd.paged import PagedCache, PagedDecoder
+    announce("paged prompts that do not fit")
+    weights = make("decoder", 22)
+    cache = PagedCache(weights.config, 3, 192, 10, 64, "cuda", page_size=16)
+    model = PagedDecoder(weights, cache)
+    roomy = PagedDecoder(weights, PagedCache(weights.config, 3, 192, 40, 64, "cuda", page_size=16))
+    held, long, other = _prompts(2, 64, 150, 5)
+    model.prefill([held, [], []])  # 4 of the 10 pages; 64 tokens of `long` take 4, 2 are left
+    with pytest.raises(RuntimeError):
+        model.prefill([[], long, other])
+    assert cache.lengths.tolist() == [64, 64, 5]
+    cache.release([0, 2])  # 6 pages, as many as the rest takes
+    got = model.prefill([[], long[64:], []])
+    assert cache.lengths.tolist() == [0, 150, 0]
+    roomy.prefill([held, [], []])
+    roomy.prefill([[], long[:64], []])
+    roomy.cache.release([0])
+    want = roomy.prefill([[], long[64:], []])
+    assert torch.equal(got[1], want[1])
