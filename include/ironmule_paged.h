@@ -68,7 +68,8 @@ typedef struct {
  * tokens), 1 not enough pages, 2 malformed (a negative count or length, more tokens than its columns,
  * a shared page past its tokens), 3 not enough rows.  Pages and rows count as asked for by every
  * well-formed request up to it, refused ones too, so the first request that does not fit ends the
- * taking of pages (of rows).  A refused request keeps its pages and gets no rows; ends[r] = lengths[r].
+ * taking of pages (of rows).  A request that is malformed for a shared page past its tokens (found while
+ * the pages are counted) counts like a well-formed one; the other malformed ones ask for nothing.  A refused request keeps its pages and gets no rows; ends[r] = lengths[r].
  * The lengths are not changed.
  * Takes the place of the admission of a request into a KV pool slot (ironmule/dense_plan.py:297-301). */
 IMQ_API int32_t imq_paged_reserve(const imq_paged_cache* cache, const int32_t* counts, const imq_paged_chunk* chunk,
