@@ -1651,7 +1651,8 @@ constexpr int64_t kCached = 256ll << 20;
 // The keys (of heads of 128) up to which tiles of few queries are left whole, one workgroup each and no second launch,
 // rather than cut into equal parts of all their blocks.  One request: 512 keys 9.3 us and 11.3 cut, 777 equal, 1024
 // 13.7 and 11.9; eight requests (64 workgroups): 512 keys 9.5 and 15.3, 1024 13.8 and 16.5, 2000 22.8
-// and 22.1; 32 requests: 1024 17.8 and 23.8, 2000 29 and 33, 4000 68 and 62.
+// and 22.1; 32 requests: 1024 17.8 and 23.8, 2000 29 and 33, 4000 68 and 62.  Longer requests of the launch fill the
+// card with theirs: their queries count as well (a prompt of 1000 tokens in tables of 2048, 25 and 27).
 int64_t rows_alone(int64_t workgroups) { return workgroups >= 128 ? 2048 : workgroups >= 32 ? 1024 : 768; }
 
 // Requests of up to kRowsMost queries go to rows_workgroup, longer ones to tile_workgroup.  The
@@ -1672,11 +1673,13 @@ AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, 
     AttendLaunch& l = p.few;
     l.width = kRowsTile;
     l.most = all_few ? INT32_MAX : kRowsMost;
-    l.tiles = with + queries / kRowsTile;  // at most one part-full tile for each request with rows
+    const int64_t all = with + queries / kRowsTile;  // of all rows: at most one part-full tile for each request
+    // (beside longer requests only those of the others are here, which have at most kRowsMost queries)
+    l.tiles = all_few ? all : std::min<int64_t>(all, (int64_t)with * (kRowsMost / kRowsTile));
     const int64_t line = l.tiles * (keys / kRowsBlock + 2);
     l.units = std::min<int64_t>(ceil_div(resident, Hkv),
                                 ceil_div(line, kRowsLeast));
-    if (keys * head_dim <= rows_alone(l.tiles * Hkv) * 128) l.units = 0;
+    if (keys * head_dim <= rows_alone(all * Hkv) * 128) l.units = 0;
     l.workgroups = l.units ? l.units : l.tiles;
     l.slots = l.units > 1 ? 2 * l.units : 0;  // a part's first tile and its last
   }
