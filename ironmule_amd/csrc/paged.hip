@@ -674,8 +674,10 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {  // v_pk_
 // blocks is cut into `units` equal parts whatever tiles they belong to, a workgroup takes one, tile
 // after tile, and each of its four wavefronts a quarter of a tile's keys there, 32 at a time.
 // Scores are K Q^T on v_mfma_f32_16x16x32_bf16, so that a lane holds keys of one query: P^T is then
-// the B operand of V^T P^T without leaving its lane (keys 4 g .. of two 16-key tiles), rounded to bf16
-// (a relative 2^-8 at most; the maxima, the sums and P V itself stay in fp32).  K goes from
+// the B operand of V^T P^T without leaving its lane (keys 4 g .. of two 16-key tiles), as two terms of bf16
+// (2^-16 of a probability are lost, as in the slots' decode attention: where values of both signs all but
+// cancel, one term's 2^-8 would be most of the result; the second product hides under the loads, 32 requests
+// of up to 8000 tokens 112.9 us and 113.1 with it, one of 777 11.5 and 11.6).  K goes from
 // its page to the A operand directly; V goes through the wavefront's own LDS by rows, 32-byte pieces
 // swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
@@ -842,9 +844,14 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
           p[b][e] = __builtin_amdgcn_exp2f(sc[b][e] - base);
           sum += p[b][e];
         }
-      const u32x4_t pw = {pack_bf16(p[0][0], p[0][1]), pack_bf16(p[0][2], p[0][3]), pack_bf16(p[1][0], p[1][1]),
-                          pack_bf16(p[1][2], p[1][3])};
-      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw);
+      u32x4_t pw, rest;  // the probabilities as two terms of bf16 each
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float even = p[i / 2][2 * (i % 2)], odd_one = p[i / 2][2 * (i % 2) + 1];
+        pw[i] = pack_bf16(even, odd_one);
+        rest[i] = pack_bf16(even - __uint_as_float(pw[i] << 16), odd_one - __uint_as_float(pw[i] & 0xffff0000u));
+      }
+      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw), pr = __builtin_bit_cast(bf16x8_t, rest);
       __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
@@ -857,6 +864,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
         const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(v0 + 16 * 2 * D));
         const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf, o[c], 0, 0, 0);
+        o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pr, o[c], 0, 0, 0);
       }
       __builtin_amdgcn_wave_barrier();
       if (__any(odd)) {
@@ -865,7 +873,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
           if (!held(b ? now1 : now0) || key < low || key > tile_last) continue;
           const float mine = b ? ((r & 2) ? ((r & 1) ? p[1][3] : p[1][2]) : ((r & 1) ? p[1][1] : p[1][0]))
                                : ((r & 2) ? ((r & 1) ? p[0][3] : p[0][2]) : ((r & 1) ? p[0][1] : p[0][0]));
-          const float pr = __shfl(mine, n + 16 * ((r >> 2) & 3));
+          const float chance = __shfl(mine, n + 16 * ((r >> 2) & 3));
           const bool seen = live && key <= position && (!a.window || key > position - a.window);
           const uint16_t* const v = a.v_pages + group_offset(b ? now1 : now0, at, b) / 2 + (r & 15) * D;
 #pragma unroll
@@ -873,7 +881,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t bits = v[16 * c + 4 * g + e];
-              if (seen && (bits & 0x7f80u) == 0x7f80u) o[c][e] += pr * bf16_bits_to_f32(bits);
+              if (seen && (bits & 0x7f80u) == 0x7f80u) o[c][e] += chance * bf16_bits_to_f32(bits);
             }
         }
       }
@@ -1085,11 +1093,12 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
 // four wavefronts 32 of them; the key blocks go through LDS, shared by the four and twice there, the loads
 // of the next one in flight over the current one's work and one barrier per block.  Scores are K Q^T on
 // v_mfma_f32_32x32x16_bf16 and P^T the B operand of V^T P^T without leaving its lane, as above (keys 4 h ..
-// and 8 + 4 h .. of 16).  The running maximum follows only when a score passes it by 2^8: until then the
-// probabilities are up to 256, which costs no accuracy, and the sums need not be scaled again.  K lies in
-// LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both swizzled so that the rows that a read takes
-// at a time lie in different banks (the 32-byte pieces of attend_rows and K's by row & 7 had every read
-// conflict once: half of the LDS cycles).
+// and 8 + 4 h .. of 16), rounded to one term of bf16 (2^-8 of it at most): a second one would be half as many
+// matrix instructions again, which bound these tiles.  The running maximum follows only when a score passes it
+// by 2^8: until then the probabilities are up to 256, which costs no accuracy, and the sums need not be scaled
+// again.  K lies in LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both swizzled so that the rows
+// that a read takes at a time lie in different banks (the 32-byte pieces of attend_rows and K's by row & 7 had
+// every read conflict once: half of the LDS cycles).
 //
 // A tile is cut into splits of at most `chunk` blocks (tile_chunk).  Tiles of requests that have several
 // splits come first, and a request's last tiles, the longest, before its first ones.
