@@ -97,8 +97,8 @@ IMQ_API int32_t imq_paged_write(const uint16_t* q, int64_t ldq, const uint16_t* 
 /* Row i of request r, at position p = ends[r] - (starts[r + 1] - starts[r]) + i, attends over its
  * request's positions max(0, p - window + 1) .. p (window 0: from 0):
  *   out[row][h] = softmax(scale q[row][h] . K[h / (Hq / Hkv)]) V[h / (Hq / Hkv)]
- * with fp32 scores, maxima and sums.  For the product with V a probability is two terms of bf16 (2^-16 of it
- * are lost, as in imq_attention_decode) for a request of up to 32 / (Hq / Hkv) new tokens, and rounded to one
+ * with fp32 scores, maxima and sums.  For the product with V a probability is two terms of bf16 (2^-15 of it
+ * are lost at most, about as in imq_attention_decode) for a request of up to 32 / (Hq / Hkv) new tokens, and rounded to one
  * (2^-8) where it has more, which are less than imq_prompt_layer keeps; in a batch whose requests have that
  * many on average all have two terms.
  * One token per request is a decode step, many a chunk of a prompt over what is cached already; a

@@ -675,9 +675,9 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {  // v_pk_
 // after tile, and each of its four wavefronts a quarter of a tile's keys there, 32 at a time.
 // Scores are K Q^T on v_mfma_f32_16x16x32_bf16, so that a lane holds keys of one query: P^T is then
 // the B operand of V^T P^T without leaving its lane (keys 4 g .. of two 16-key tiles), as two terms of bf16
-// (2^-16 of a probability are lost, as in the slots' decode attention: where values of both signs all but
-// cancel, one term's 2^-8 would be most of the result; the second product hides under the loads, 32 requests
-// of up to 8000 tokens 112.9 us and 113.1 with it, one of 777 11.5 and 11.6).  K goes from
+// (2^-15 of a probability are lost, about as in the slots' decode attention: where values of both signs all
+// but cancel, one term's 2^-8 would be most of the result; the second product hides under the loads, 32
+// requests of up to 8000 tokens 113.8 us and 114.2 with it, one of 777 11.5 and 11.6).  K goes from
 // its page to the A operand directly; V goes through the wavefront's own LDS by rows, 32-byte pieces
 // swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
@@ -844,12 +844,17 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, int head, const
           p[b][e] = __builtin_amdgcn_exp2f(sc[b][e] - base);
           sum += p[b][e];
         }
-      u32x4_t pw, rest;  // the probabilities as two terms of bf16 each
+      // The probabilities as two terms of bf16 each: the first cut off, the second what is left and 2^-20 of it all
+      // (which scales every output alike), so that it is above zero where the first one is: an infinite value times
+      // a zero or a negative number would be a NaN, or one with the first product.
+      u32x4_t pw, rest;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float even = p[i / 2][2 * (i % 2)], odd_one = p[i / 2][2 * (i % 2) + 1];
-        pw[i] = pack_bf16(even, odd_one);
-        rest[i] = pack_bf16(even - __uint_as_float(pw[i] << 16), odd_one - __uint_as_float(pw[i] & 0xffff0000u));
+        const uint32_t e = __float_as_uint(even), o1 = __float_as_uint(odd_one);
+        pw[i] = __builtin_amdgcn_perm(o1, e, 0x07060302);
+        rest[i] = pack_bf16(fmaf(even, 1.0f + 0x1p-20f, -__uint_as_float(e & 0xffff0000u)),
+                            fmaf(odd_one, 1.0f + 0x1p-20f, -__uint_as_float(o1 & 0xffff0000u)));
       }
       const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, pw), pr = __builtin_bit_cast(bf16x8_t, rest);
       __builtin_amdgcn_wave_barrier();  // (a wavefront's LDS accesses complete in order)

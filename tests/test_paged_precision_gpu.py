@@ -1,5 +1,5 @@
-"""The probabilities of steps and short chunks over pages keep 16 bits for the product with the values, as those
-of the slots' decode attention do: values of both signs that all but cancel show what is lost."""
+"""The probabilities of steps and short chunks over pages are two terms of bf16 for the product with the values, as
+those of the slots' decode attention are: values of both signs that all but cancel show what is lost."""
 
 from __future__ import annotations
 
@@ -23,8 +23,10 @@ WEIGHT = 129 / 256
     [(1, 900), (300, 300), (8, 64)]])
 def test_sums_that_cancel(dim, requests):
     """Every other key scores DELTA less and its values are the others' over -WEIGHT: the output is a thousandth of
-    the values, and nothing if the probability is rounded to bf16.  Two terms of bf16 leave 2^-16 of a
-    probability; the rest of the bound as in paged_model.attention, of values up to 1."""
+    the values, and nothing if the probability is rounded to bf16.  The first term has a probability's upper eight
+    bits, cut off: less than 2^-7 of it is left (8 bits, the first one 1), of which the second term's rounding
+    takes half a step, 2^-8 of that at most: 2^-15.  The 2^-20 that is added scales the whole output (2^-20 of it,
+    within its rounding's 2^-8).  The rest of the bound as in paged_model.attention, of values up to 1."""
     import torch
 
     from ironmule_amd import _native
@@ -43,7 +45,7 @@ def test_sums_that_cancel(dim, requests):
     b.run(_native)
     want, _ = attention(torch, b.q, b.k, b.v, b.tables, b.starts, b.ends, 1.0)
     u, longest = 2.0 ** -24, max(end for _, end in requests)
-    rest = 2.0 ** -16 + 2 * (dim + 8) * u * DELTA + 2 * (longest / 16 + 64) * u
+    rest = 2.0 ** -15 + 2 * (dim + 8) * u * DELTA + 2 * (longest / 16 + 64) * u
     starts = b.starts.tolist()
     for r, (n, _) in enumerate(requests):
         if 4 * n > 32:
