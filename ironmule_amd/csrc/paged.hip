@@ -682,9 +682,9 @@ __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {  // v_pk_
 // swizzled, and is read transposed.  The next block's K loads are issued as soon as this block's are
 // used, its V loads when this block's have gone to LDS: 16 KB (head size 128) in flight per wavefront
 // over the softmax and P V, and no barrier before the wavefronts' results are joined.
-// Bound by memory: 32 requests of up to 8000 tokens, 32 heads on 8 of 128 (669 MB), in 109 us, 6.1 TB/s, and 6 us
-// for the second launch.  One of 777 tokens 7.4 and 4.8 us: the chain of starts, lengths, table and keys, each
-// a load after the last.  Parts of four blocks: a request of 8000 tokens 17 us instead of 14.
+// Bound by memory: 32 requests of up to 8000 tokens, 32 heads on 8 of 128 (669 MB), in 110 us, 6.1 TB/s, and 5 us
+// for the second launch; 16 heads on 8 of 256 (1.33 GB) in 211 us with it, 6.3 TB/s.  One of 777 tokens 7.8 and
+// 5.0 us: the chain of starts, lengths, table and keys, each a load after the last.  Parts of four blocks: a request of 8000 tokens 17 us instead of 14.
 constexpr int kRowsTile = 16, kRowsBlock = 32, kRowsLeast = 8;
 constexpr int kRowsMost = 32;  // queries of a request that rows_workgroup is there for
 template <int D>
@@ -1098,8 +1098,9 @@ __device__ __forceinline__ void merge_rows(const AttendArgs& a, int index, Merge
 // four wavefronts 32 of them; the key blocks go through LDS, shared by the four and twice there, the loads
 // of the next one in flight over the current one's work and one barrier per block.  Scores are K Q^T on
 // v_mfma_f32_32x32x16_bf16 and P^T the B operand of V^T P^T without leaving its lane, as above (keys 4 h ..
-// and 8 + 4 h .. of 16), rounded to one term of bf16 (2^-8 of it at most): a second one would be half as many
-// matrix instructions again, which bound these tiles.  The running maximum follows only when a score passes it
+// and 8 + 4 h .. of 16), rounded to one term of bf16 (2^-8 of it at most): a second one is half as many
+// matrix instructions again, which bound these tiles (1024 tokens of 16384: 272 us, and 375 with it; heads
+// of 256 with windows 53 and 63).  The running maximum follows only when a score passes it
 // by 2^8: until then the probabilities are up to 256, which costs no accuracy, and the sums need not be scaled
 // again.  K lies in LDS by rows of 16-byte pieces, V by rows of 64-byte ones, both swizzled so that the rows
 // that a read takes at a time lie in different banks (the 32-byte pieces of attend_rows and K's by row & 7 had
@@ -1670,7 +1671,8 @@ constexpr int64_t kCached = 256ll << 20;
 int64_t rows_alone(int64_t workgroups) { return workgroups >= 128 ? 2048 : workgroups >= 32 ? 1024 : 768; }
 
 // Requests of up to kRowsMost queries go to rows_workgroup, longer ones to tile_workgroup.  The
-// host knows the sums only: where the average request stays within kRowsMost the first serves all.
+// host knows the sums only: where the average request stays within kRowsMost the first serves all, a chunk among
+// many steps too (63 steps and a chunk of 449 tokens, all over 8000, 539 us; 323 and 96 in calls of their own).
 // A workgroup with nothing to do costs its launch all the same (1000 of them 10 us): no more are launched than
 // the longest context can give work to.  The device makes do with what there is, whatever the contexts.
 AttendPlan plan_attend(int32_t rows, int32_t requests, int32_t Hq, int32_t Hkv, int32_t head_dim, int64_t max_context,

@@ -164,8 +164,9 @@ class PagedDecoder:
         tokens: lists of numbers per request, or an int32 tensor (requests, width) on the GPU with counts
         there too; then `rows` bounds the sum of the counts (default: the cache's rows, or requests *
         width if that is less), and a request with a count past its tokens is refused (status 2).  max_context
-        bounds the requests' lengths and only plans the launches.  A token outside the vocabulary makes its
-        request's logits NaN from then on."""
+        bounds the requests' lengths and only plans the launches (default: what the cache's tables can hold;
+        short contexts in a large cache are faster with their own bound).  A token outside the vocabulary makes
+        its request's logits NaN from then on."""
         c, cache = self.weights.config, self.cache
         device, limits = cache.pool.device, None
         if not isinstance(tokens, torch.Tensor):
@@ -280,9 +281,9 @@ class PagedDecoder:
     def beam_search(self, prompts, beams: int, steps: int, eos: int = -1):
         """The `beams` continuations of up to `steps` tokens that beam search finds for each prompt: (tokens
         int32 (prompts, beams, steps), scores fp32 (prompts, beams): the sums of their log probabilities,
-        the best first).  A continuation ends with token `eos` (-1: none does), which fills what is left of it; where
-        there are fewer than `beams` continuations the tokens are -1, the score -inf.  The cache has
-        len(prompts) * beams requests, which are ended first; the beams' requests are left in it, without
+        the best first).  A continuation ends with token `eos` (-1: none does), which fills what is left of
+        it (every step is launched all the same, as nothing waits for the tokens); where there are fewer than
+        `beams` continuations the tokens are -1, the score -inf.  The cache has len(prompts) * beams requests, which are ended first; the beams' requests are left in it, without
         their last tokens.  Raises RuntimeError if the cache has not the pages."""
         cache, groups = self.cache, len(prompts)
         if groups < 1 or beams < 1 or groups * beams != cache.requests:
